@@ -1,6 +1,7 @@
 """cube_awq_b200 — B200 (sm_100a) implementation of the AWQ INT4 hot path of
 joshuawm/cube-awq: the fused dequant-GEMM (decode and prefill kernels) and the
-standalone dequantize kernel, behind the reference's module API.
+standalone dequantize kernel, behind the reference's module API; and the
+operators between the linears of a decoder layer (``layer_ops``).
 
     from cube_awq_b200 import AWQGEMMLinearConfig
     layer = AWQGEMMLinearConfig(4096, 4096, 128).with_bias(False).build("cuda:0", torch.float16)
@@ -21,6 +22,8 @@ from .kernel import (DECODE_M_THRESHOLD, DECODE_TILE_M, ShapeConfig, autotune, a
                      gemm_silu_mul, interleave_gate_up, plan_cache_clear, plan_get, plan_set,
                      select_tile_m, select_tile_n, validate_decode_launch_params,
                      validate_launch_params, version)
+from .layer_ops import (attention_decode, attention_prefill, rms_norm, rms_norm_fp8, rope_append,
+                        rope_table)
 from .modules import (AWQGateUpSiluMul, AWQGEMMLinear, AWQGEMMLinearConfig, AWQLinear,
                       AWQLinearConfig, AWQQKVLinear)
 from .tp import ColumnParallelAWQLinear, RowParallelAWQLinear, TPComm, TPPeers
@@ -45,6 +48,8 @@ __all__ = [
     "DECODE_M_THRESHOLD", "DECODE_TILE_M", "ShapeConfig", "autotune", "awq_gemm_linear",
     "dequantize_awq", "dequantize_native", "device_error", "gemm", "gemm_qkv", "gemm_silu_mul",
     "interleave_gate_up", "plan_cache_clear",
+    "attention_decode", "attention_prefill", "rms_norm", "rms_norm_fp8", "rope_append",
+    "rope_table",
     "plan_get", "plan_set", "select_tile_m", "select_tile_n", "validate_decode_launch_params",
     "validate_launch_params", "version",
 ]

@@ -45,6 +45,8 @@ EXPORTED = (
     "cawq_gemm_qkv",
     "cawq_plan_get", "cawq_plan_set", "cawq_plan_cache_clear", "cawq_autotune",
     "cawq_dequantize_native", "cawq_dequantize",
+    "cawq_rms_norm", "cawq_rms_norm_fp8", "cawq_rope_append", "cawq_attention_workspace",
+    "cawq_attention_decode", "cawq_attention_prefill",
     "cawq_tp_column_shard", "cawq_tp_row_shard", "cawq_tp_interleave_columns",
     "cawq_tp_unique_id", "cawq_tp_init", "cawq_tp_destroy", "cawq_tp_info",
     "cawq_gemm_colpar", "cawq_gemm_rowpar", "cawq_gemm_rowpar_noalloc",
@@ -63,6 +65,17 @@ class PeersC(ctypes.Structure):
     _fields_ = [("world", ctypes.c_int), ("rank", ctypes.c_int),
                 ("base", ctypes.c_void_p * CAWQ_TP_MAX_PEERS), ("bytes", ctypes.c_size_t),
                 ("timeout_ms", ctypes.c_int)]
+
+
+class PagedKVC(ctypes.Structure):
+    """cawq_paged_kv: a paged key / value cache and the batch of a call."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("pages", ctypes.c_size_t),
+                ("n_kv", ctypes.c_size_t), ("page_size", ctypes.c_size_t),
+                ("head_dim", ctypes.c_size_t), ("stride_page", ctypes.c_size_t),
+                ("stride_head", ctypes.c_size_t), ("stride_token", ctypes.c_size_t),
+                ("block_table", ctypes.c_void_p), ("batch", ctypes.c_size_t),
+                ("table_width", ctypes.c_size_t), ("ld_table", ctypes.c_size_t),
+                ("seq_lens", ctypes.c_void_p), ("q_start", ctypes.c_void_p)]
 
 
 class ShapeConfigC(ctypes.Structure):
@@ -152,6 +165,19 @@ def _declare(L) -> None:
     L.cawq_dequantize_native.restype = st
     L.cawq_dequantize.argtypes = [u32p, u32p, vp, vp, sz, sz, sz, i, i, vp]
     L.cawq_dequantize.restype = st
+    f32, kv_p = ctypes.c_float, ctypes.POINTER(PagedKVC)
+    L.cawq_rms_norm.argtypes = [vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, f32, i, vp]
+    L.cawq_rms_norm.restype = st
+    L.cawq_rms_norm_fp8.argtypes = [vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, f32, i, vp]
+    L.cawq_rms_norm_fp8.restype = st
+    L.cawq_rope_append.argtypes = [vp, vp, vp, vp, sz, vp, kv_p, sz, sz, sz, sz, sz, sz, i, vp]
+    L.cawq_rope_append.restype = st
+    L.cawq_attention_workspace.argtypes = [kv_p, sz, sz]
+    L.cawq_attention_workspace.restype = sz
+    L.cawq_attention_decode.argtypes = [vp, vp, kv_p, sz, sz, sz, f32, sz, sz, i, vp, sz, vp]
+    L.cawq_attention_decode.restype = st
+    L.cawq_attention_prefill.argtypes = [vp, vp, kv_p, sz, sz, sz, sz, f32, sz, sz, i, vp, sz, vp]
+    L.cawq_attention_prefill.restype = st
     L.cawq_tp_column_shard.argtypes = [sz, i, i, ctypes.POINTER(sz), ctypes.POINTER(sz)]
     L.cawq_tp_column_shard.restype = st
     L.cawq_tp_row_shard.argtypes = [sz, sz, i, i, ctypes.POINTER(sz), ctypes.POINTER(sz)]

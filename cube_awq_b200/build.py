@@ -27,7 +27,7 @@ REPO = os.path.dirname(PKG_DIR)
 INCLUDE = os.path.join(REPO, "include")
 LIB_PATH = os.path.join(PKG_DIR, "libcube_awq.so")
 
-SOURCES = ["cawq_api.cu", "cawq_kernels.cu"]
+SOURCES = ["cawq_api.cu", "cawq_kernels.cu", "cawq_layer.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -41,7 +41,7 @@ cawq_status cuda_fail(cudaError_t e, const char* where) {
   return fail(CAWQ_ERR_CUDA, m);
 }
 
-static std::string fmt(const char* f, ...) {
+std::string fmt(const char* f, ...) {
   char buf[512];
   va_list ap;
   va_start(ap, f);
@@ -84,7 +84,7 @@ cawq_status current_device_info(DeviceInfo* info) {
   return CAWQ_OK;
 }
 
-static cawq_status require_sm100(DeviceInfo* dev) {
+cawq_status require_sm100(DeviceInfo* dev) {
   cawq_status st = current_device_info(dev);
   if (st != CAWQ_OK) return st;
   if (dev->cc_major != 10) {

@@ -78,8 +78,23 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
 
 // ------------------------------------------------- device error word
 // Bit 0: a bounded wait (mbarrier / cluster) gave up. Host reads it through
-// cawq_device_error(). Defined here: only cawq_kernels.cu includes this file.
-__device__ uint32_t g_cawq_device_error = 0;
+// cawq_device_error(), which joins the words of the translation units that
+// include this file (each has its own).
+static __device__ uint32_t g_cawq_device_error = 0;
+
+// Adds this translation unit's word to *word (and clears it with reset); the
+// caller has synchronised the device.
+static inline cudaError_t read_own_error_word(uint32_t* word, int reset) {
+  uint32_t own = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&own, g_cawq_device_error, sizeof(uint32_t));
+  if (e != cudaSuccess) return e;
+  *word |= own;
+  if (reset) {
+    const uint32_t zero = 0;
+    e = cudaMemcpyToSymbol(g_cawq_device_error, &zero, sizeof(uint32_t));
+  }
+  return e;
+}
 
 __device__ __forceinline__ uint64_t globaltimer_ns() {
   uint64_t t;

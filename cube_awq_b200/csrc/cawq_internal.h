@@ -59,6 +59,9 @@ struct DeviceInfo {
   size_t smem_optin = 0;
 };
 cawq_status current_device_info(DeviceInfo* info);
+// the same, and CAWQ_ERR_UNSUPPORTED unless it is an sm_100 device
+cawq_status require_sm100(DeviceInfo* dev);
+std::string fmt(const char* f, ...);
 
 // Driver entry point for cuTensorMapEncodeTiled (resolved through the runtime,
 // so the library needs no -lcuda).
@@ -156,5 +159,7 @@ cudaError_t launch_p2p_rowpar_finish(const P2PSync& s, const float* slot, const 
 cudaError_t rowpar_static_scratch(float** ptr);
 
 cudaError_t read_device_error(uint32_t* word, int reset);
+// cawq_layer.cu's part of it (after a device synchronisation)
+cudaError_t read_layer_error(uint32_t* word, int reset);
 
 }  // namespace cawq

@@ -1,5 +1,6 @@
-// cawq_kernels.cu — the device code of libcube_awq.so, one translation unit so
-// every kernel shares the device error word without relocatable device code.
+// cawq_kernels.cu — the GEMM, dequantize and tensor-parallel kernels of
+// libcube_awq.so, one translation unit so they share a device error word
+// without relocatable device code (cawq_layer.cu has the other one).
 #include "cawq_common.cuh"
 
 namespace cawq {
@@ -7,13 +8,9 @@ namespace cawq {
 cudaError_t read_device_error(uint32_t* word, int reset) {
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return e;
-  e = cudaMemcpyFromSymbol(word, g_cawq_device_error, sizeof(uint32_t));
-  if (e != cudaSuccess) return e;
-  if (reset) {
-    const uint32_t zero = 0;
-    e = cudaMemcpyToSymbol(g_cawq_device_error, &zero, sizeof(uint32_t));
-  }
-  return e;
+  *word = 0;
+  if ((e = read_own_error_word(word, reset)) != cudaSuccess) return e;
+  return read_layer_error(word, reset);
 }
 
 }  // namespace cawq

@@ -141,7 +141,8 @@ int cawq_device_supported(int device);
 /*
  * Reads (and with reset != 0 clears) the device-side error word of the
  * current device: bit 0 = a bounded wait inside a kernel timed out; bit 1 =
- * a fused tensor-parallel call gave up waiting for a peer's flag.
+ * a fused tensor-parallel call gave up waiting for a peer's flag; bit 2 = a
+ * call on a paged cache skipped a page or position outside it.
  * Synchronises the device.
  */
 cawq_status cawq_device_error(int reset, uint32_t* word);
@@ -331,6 +332,105 @@ cawq_status cawq_dequantize(const uint32_t* qweight, const uint32_t* qzeros,
                             const void* scales, void* out, size_t k, size_t n,
                             size_t group_size, cawq_dtype dtype,
                             cawq_order order, void* stream);
+
+/* ----------------------------------------------------------------------- */
+/* Between the linears of a decoder layer (no reference counterpart: its   */
+/* decoder leaves them to the host framework)                              */
+/* ----------------------------------------------------------------------- */
+
+/*
+ * RMS norm with the residual's addition, row by row:
+ *   h = x + residual (h = x when residual is NULL), kept in fp32;
+ *   residual_out = h rounded to `dtype` (with a residual only; may be the
+ *   residual's own buffer, or NULL);
+ *   y = h / sqrt(mean(h^2) + eps) * weight, rounded once to `dtype`.
+ * x, residual, y and residual_out are [rows, d] with row strides in elements
+ * (0 = d); weight is [d]. y may be x's own buffer. eps >= 0.
+ */
+cawq_status cawq_rms_norm(const void* x, const void* weight, const void* residual, void* y,
+                          void* residual_out, size_t rows, size_t d, size_t ld_x,
+                          size_t ld_residual, size_t ld_y, size_t ld_residual_out, float eps,
+                          cawq_dtype dtype, void* stream);
+
+/*
+ * The same with y in 8 bits: scales[row] = max |y| / 448 (fp32) and
+ * y8 = e4m3(y / scales[row]), rounded to nearest even from the fp32 y; a row
+ * of zeros has scale 0. y8 must not overlap x.
+ */
+cawq_status cawq_rms_norm_fp8(const void* x, const void* weight, const void* residual, void* y8,
+                              float* scales, void* residual_out, size_t rows, size_t d,
+                              size_t ld_x, size_t ld_residual, size_t ld_y8,
+                              size_t ld_residual_out, float eps, cawq_dtype dtype, void* stream);
+
+/*
+ * A paged key / value cache and the batch that a call works on. Row (page,
+ * head, slot) of k and v starts at page * stride_page + head * stride_head +
+ * slot * stride_token elements and holds head_dim elements; k and v have the
+ * same strides (multiples of 8 elements, base pointers 16-byte aligned).
+ * Token j of sequence b lies in page block_table[b * ld_table + j / page_size],
+ * slot j % page_size. seq_lens[b] counts the tokens of sequence b with the
+ * call's own; its new tokens are rows q_start[b] .. q_start[b + 1] - 1 of the
+ * call's tensors and its last ones: new token i of n is at position
+ * seq_lens[b] - n + i. q_start NULL: one new token per sequence.
+ * seq_lens, q_start and block_table are device memory, so their values are
+ * checked by the kernels: a page outside [0, pages) or a position past the
+ * table is skipped (no read, no write) and sets bit 2 of the device error
+ * word; a new token whose position is negative (an empty slot of a batch)
+ * sees no key.
+ */
+typedef struct cawq_paged_kv {
+  void* k;
+  void* v;
+  size_t pages, n_kv, page_size, head_dim; /* page_size % 8 == 0; head_dim 64 or 128 */
+  size_t stride_page, stride_head, stride_token;
+  const int32_t* block_table; /* [batch, table_width], row stride ld_table */
+  size_t batch, table_width, ld_table;
+  const int32_t* seq_lens; /* [batch] */
+  const int32_t* q_start;  /* [batch + 1], ascending from 0 to the row count, or NULL */
+} cawq_paged_kv;
+
+/*
+ * Rotary embedding of the new tokens' q and k and the append of k and v to
+ * the cache, in one launch. q [tokens, n_q, head_dim], k and v [tokens, n_kv,
+ * head_dim] (heads dense, token strides in elements, 0 = dense); rope is fp32
+ * [rope_rows, head_dim]: row p holds the head_dim / 2 cosines, then the sines,
+ * of position p, and element i turns with element i + head_dim / 2. q_out may
+ * be q's own buffer. Rounded once to `dtype` (CAWQ_F16 or CAWQ_BF16). A token
+ * with a negative position gets a zero q_out and no place in the cache; one at
+ * or past rope_rows the same, with bit 2 of the device error word.
+ */
+cawq_status cawq_rope_append(const void* q, const void* k, const void* v, const float* rope,
+                             size_t rope_rows, void* q_out, const cawq_paged_kv* kv,
+                             size_t tokens, size_t n_q, size_t ld_q, size_t ld_k, size_t ld_v,
+                             size_t ld_q_out, cawq_dtype dtype, void* stream);
+
+/*
+ * Attention of the new tokens over the cache that already holds them:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j
+ * over the visible positions j of the token's sequence: j <= pos, and with
+ * window > 0 also j > pos - window or j < sinks (the first `sinks` tokens
+ * stay visible). Query head h reads kv head h / (n_q / n_kv). A token that
+ * sees nothing gets zeros. Scores, the running maximum and sum and the output
+ * sums are fp32; the weights of the second product are rounded to `dtype`.
+ * q and out: [tokens, n_q, head_dim], token strides in elements (0 = dense),
+ * CAWQ_F16 or CAWQ_BF16. workspace: cawq_attention_workspace() bytes of device
+ * memory, 16-byte aligned, that no other call uses while this one runs.
+ *
+ * cawq_attention_decode: one token per sequence (tokens = kv->batch, q_start
+ * unused). cawq_attention_prefill: any number per sequence (q_start required);
+ * rows of `out` that belong to no sequence are left as they are.
+ */
+size_t cawq_attention_workspace(const cawq_paged_kv* kv, size_t tokens, size_t n_q);
+
+cawq_status cawq_attention_decode(const void* q, void* out, const cawq_paged_kv* kv, size_t n_q,
+                                  size_t ld_q, size_t ld_out, float scale, size_t window,
+                                  size_t sinks, cawq_dtype dtype, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+cawq_status cawq_attention_prefill(const void* q, void* out, const cawq_paged_kv* kv,
+                                   size_t tokens, size_t n_q, size_t ld_q, size_t ld_out,
+                                   float scale, size_t window, size_t sinks, cawq_dtype dtype,
+                                   void* workspace, size_t workspace_bytes, void* stream);
 
 /* ----------------------------------------------------------------------- */
 /* Tensor-parallel helpers (no reference counterpart: the reference is     */
