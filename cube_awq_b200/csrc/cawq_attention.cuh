@@ -1,79 +1,665 @@
-// cawq_attention.cuh — attention of new tokens over a paged cache (sm_100a).
+// cawq_attention.cuh — attention of few query rows over a paged cache, split
+// over the cache's length (sm_100a): one new token per sequence, or short runs
+// of them.
 //
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(s_j - m),  s_j = scale log2(e) q . k_j
 //
-// over the visible positions, m their running maximum. One warp per (token,
-// query head); the lanes hold the head's dimensions and the keys pass one by
-// one.
+// over the visible positions, m their running maximum. Two parts with their
+// own maxima join exactly: with M = max(m1, m2), sum = 2^(m1 - M) sum1 +
+// 2^(m2 - M) sum2, the same for the outputs.
+//
+// Bound by the cache's bytes: every visible key and value is read once per
+// tile of query rows that shares its kv head. A row tile is NR = 8 or 16 rows
+// of one (sequence, kv head): the G = n_q / n_kv query heads of its tokens,
+// token by token. All (row tile, 64-key tile) units of the batch, sequences of
+// any length, form one list that is dealt out evenly to a grid of two CTAs per
+// SM, so a batch of ragged lengths and one long sequence fill the GPU alike;
+// the lengths are read on the device. A CTA's share may begin or end inside a
+// row tile's keys: it then leaves its part (m, sum, outputs, fp32) in the
+// workspace and a second small kernel joins the parts in order (no atomics:
+// the same bits every time).
+//
+// A CTA is four warps that never wait for one another inside a row tile: warp
+// w takes keys 16 w .. 16 w + 15 of each 64-key tile and streams them through
+// a ring of its own in shared memory (cp.async, 16 bytes a lane, rows swizzled
+// so that ldmatrix reads without bank conflicts; a masked row is filled with
+// zeros and never read). The stream runs on across row tiles. With mma.sync
+// m16n8k16 the keys are the MMA's rows: S^T = K Q^T needs only N = 8 columns
+// for 8 query rows; the weights, rounded to the operand type, turn in
+// registers (movmatrix) into the B operand of O^T += V^T P^T.
 #pragma once
 
+#include "cawq_norm.cuh"
 #include "cawq_paged.cuh"
 
 namespace cawq {
 
-template <int DT, int D>
-__global__ void __launch_bounds__(128)
-    attention_kernel(const char* q, char* out, const PagedView kv, uint32_t tokens, uint32_t n_q,
-                     int64_t ld_q, int64_t ld_o, float scale_log2, int window, int sinks) {
-  using T = typename DType<DT>::T;
-  constexpr int E = D / 32;
-  const uint64_t w = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (w >= (uint64_t)tokens * n_q) return;
-  const uint32_t t = static_cast<uint32_t>(w / n_q), h = static_cast<uint32_t>(w % n_q);
-  const int lane = threadIdx.x & 31;
-  const uint32_t b = kv.sequence(t);
-  if (b >= kv.batch) return;
-  int first, count;
-  kv.rows(b, tokens, &first, &count);
-  const int pos = kv.len(b) - count + static_cast<int>(t) - first;
-  const uint32_t hk = h / (n_q / kv.n_kv);
-  float qf[E], o[E];
-  const T* qr = reinterpret_cast<const T*>(q + t * ld_q + (int64_t)h * D * 2) + lane * E;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    qf[i] = DType<DT>::to_f32(qr[i]) * scale_log2;
-    o[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  const int start = window > 0 ? max(0, pos - window + 1) : 0;
-  for (int j = start > 0 && sinks > 0 ? 0 : start; j <= pos; ++j) {
-    if (j >= sinks && j < start) j = start;
-    const int64_t at = kv.offset(b, hk, static_cast<uint32_t>(j));
-    if (at < 0) continue;
-    const T* kr = reinterpret_cast<const T*>(kv.k + at) + lane * E;
-    const T* vr = reinterpret_cast<const T*>(kv.v + at) + lane * E;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) s += qf[i] * DType<DT>::to_f32(kr[i]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float mn = fmaxf(m, s);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float c = exp2f(m - base), p = exp2f(s - base);
-    l = l * c + p;
-#pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = o[i] * c + p * DType<DT>::to_f32(vr[i]);
-    m = mn;
-  }
-  T* orow = reinterpret_cast<T*>(out + t * ld_o + (int64_t)h * D * 2) + lane * E;
-#pragma unroll
-  for (int i = 0; i < E; ++i) orow[i] = DType<DT>::from_f32(l != 0.f ? o[i] / l : 0.f);
+constexpr int kAttWarps = 4;
+constexpr int kAttKeys = 16 * kAttWarps;  // keys of a unit
+constexpr int kAttStages = 3;
+constexpr int kAttMaxCtas = 320;  // most CTAs of a launch (two per SM)
+
+template <int D>
+struct AttLayout {
+  static constexpr int kRow = 2 * D;            // bytes of a key
+  static constexpr int kStage = 2 * 16 * kRow;  // keys and values of 16 positions
+  static constexpr int kRing = kAttWarps * kAttStages * kStage;
+  static constexpr int kPad = D + 4;  // floats of a merge row: 2 kPad = 8 (mod 32) banks
+  static constexpr int kMerge = kAttWarps * 8 * kPad * 4;
+  static constexpr int kSmem = kRing + kMerge;
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-cudaError_t launch_attention(const AttentionProblem& p, const PagedView& kv) {
-  const dim3 grid(static_cast<uint32_t>((p.tokens * p.n_q + 3) / 4));
-#define CAWQ_ATT(DT, D)                                                                        \
-  attention_kernel<DT, D><<<grid, 128, 0, p.stream>>>(                                         \
-      static_cast<const char*>(p.q), static_cast<char*>(p.out), kv,                            \
-      static_cast<uint32_t>(p.tokens), static_cast<uint32_t>(p.n_q), (int64_t)p.ld_q * 2,      \
-      (int64_t)p.ld_out * 2, p.scale * 1.4426950408889634f, p.window, p.sinks)
-  if (p.dtype == kF16) {
-    if (p.d == 64) CAWQ_ATT(kF16, 64); else CAWQ_ATT(kF16, 128);
+// 16 bytes global -> shared; zeros when `bytes` is 0 (nothing is read then).
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// 8x8 b16 matrix transposed across the warp: lane (g, t) gives elements
+// (g, 2t), (g, 2t + 1) and receives (2t, g), (2t + 1, g).
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (DT == kBF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    r = *reinterpret_cast<const uint32_t*>(&v);
   } else {
-    if (p.d == 64) CAWQ_ATT(kBF16, 64); else CAWQ_ATT(kBF16, 128);
+    const __half2 v = __floats2half2_rn(lo, hi);
+    r = *reinterpret_cast<const uint32_t*>(&v);
   }
+  return r;
+}
+
+// What a launch works on; both kernels walk the same list of units.
+struct AttWork {
+  PagedView kv;
+  uint32_t tokens, group, row_tile;  // group = n_q / n_kv, row_tile = NR
+  FastDiv by_group;
+  int window, sinks;
+
+  // Sequence b: its rows, its keys in order of position without the hidden
+  // ones between the sinks and the window of its first new token, and its
+  // units (64-key tiles x kv heads x row tiles). A sequence with new tokens
+  // and no keys has one tile per row tile all the same: its rows are zeros.
+  struct Seq {
+    int first, count, len, start, head, keys;
+    uint32_t tiles, row_tiles;
+    __device__ __forceinline__ int key(int c) const { return c < head ? c : c - head + start; }
+  };
+  __device__ __forceinline__ Seq seq(uint32_t b) const {
+    Seq s;
+    kv.rows(b, tokens, &s.first, &s.count);
+    s.len = kv.len(b);
+    const int pos = s.len - s.count;  // of the first new token
+    s.start = window > 0 ? max(0, pos - window + 1) : 0;
+    s.head = min(sinks, s.start);
+    s.keys = s.len - s.start + s.head;
+    s.row_tiles = (static_cast<uint32_t>(s.count) * group + row_tile - 1) / row_tile;
+    s.tiles = s.count > 0 ? max(1, (s.keys + kAttKeys - 1) / kAttKeys) : 0u;
+    return s;
+  }
+  __device__ __forceinline__ uint64_t units(const Seq& s) const {
+    return static_cast<uint64_t>(s.tiles) * s.row_tiles * kv.n_kv;
+  }
+};
+
+// Exclusive prefix sums of the sequences' units by blocks of 32 * kAttWarps
+// consecutive ones. find() leaves, in shared memory, the sequence that holds
+// unit u and its first unit; total() the number of units.
+struct AttScan {
+  uint64_t part[32 * kAttWarps];  // units before thread i's sequences
+  uint64_t sums[kAttWarps];       // of the warps
+  uint64_t total, before;
+  uint32_t seq;
+};
+
+__device__ __forceinline__ void att_scan(const AttWork& w, AttScan& sc) {
+  const uint32_t per = (w.kv.batch + 32 * kAttWarps - 1) / (32 * kAttWarps);
+  const uint32_t b0 = threadIdx.x * per, b1 = min(w.kv.batch, b0 + per);
+  uint64_t n = 0;
+  for (uint32_t b = b0; b < b1; ++b) n += w.units(w.seq(b));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint64_t inc = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) sc.sums[warp] = inc;
+  __syncthreads();
+  uint64_t base = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kAttWarps; ++i) {
+    if (i < warp) base += sc.sums[i];
+    all += sc.sums[i];
+  }
+  sc.part[threadIdx.x] = base + inc - n;
+  if (threadIdx.x == 0) sc.total = all;
+  __syncthreads();
+}
+
+// After att_scan: the sequence that holds unit u (< total) and the units before it.
+__device__ __forceinline__ void att_find(const AttWork& w, AttScan& sc, uint64_t u) {
+  const uint32_t per = (w.kv.batch + 32 * kAttWarps - 1) / (32 * kAttWarps);
+  const uint64_t lo = sc.part[threadIdx.x];
+  const uint64_t hi = threadIdx.x + 1 < 32 * kAttWarps ? sc.part[threadIdx.x + 1] : sc.total;
+  if (u >= lo && u < hi) {
+    uint64_t at = lo;
+    uint32_t b = threadIdx.x * per;
+    for (;; ++b) {
+      const uint64_t n = w.units(w.seq(b));
+      if (u < at + n) break;
+      at += n;
+    }
+    sc.seq = b;
+    sc.before = at;
+  }
+  __syncthreads();
+}
+
+// CTA c of n works on units [first(c), first(c + 1)); n is at most the number
+// of units, so that no CTA between two of a row tile's is without a part.
+__device__ __forceinline__ uint32_t att_ctas(uint64_t total, uint32_t launched) {
+  return static_cast<uint32_t>(min(total, static_cast<uint64_t>(launched)));
+}
+__device__ __forceinline__ uint64_t att_first_unit(uint64_t total, uint32_t cta, uint32_t ctas) {
+  return total * cta / ctas;
+}
+
+// A part in the workspace: NR maxima, NR sums, NR x D outputs.
+template <int D, int NR>
+__device__ __forceinline__ float* att_slot(float* ws, uint32_t slot) {
+  return ws + static_cast<size_t>(slot) * NR * (D + 2);
+}
+
+// MULTI: sequences may have several new tokens, so rows of a tile see
+// different keys. Without it every visible key is every row's.
+template <int DT, int D, int NT, bool MULTI>
+__global__ void __launch_bounds__(32 * kAttWarps, 2)
+    attention_split_kernel(const char* q, char* out, const AttWork w, int64_t ld_q, int64_t ld_o,
+                           float scale_log2, float* ws) {
+  using T = typename DType<DT>::T;
+  using L = AttLayout<D>;
+  constexpr int NR = 8 * NT, KS = D / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  AttScan& sc = *reinterpret_cast<AttScan*>(smem + L::kRing);  // read before the first merge
+  __shared__ float s_m[kAttWarps][NR], s_l[kAttWarps][NR];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t4 = lane & 3;
+
+  pdl_wait();
+  pdl_launch_dependents();  // after the wait: the joining kernel may read the lengths at once
+  att_scan(w, sc);
+  const uint32_t ctas = att_ctas(sc.total, gridDim.x);
+  if (blockIdx.x >= ctas) return;
+  const uint64_t u0 = att_first_unit(sc.total, blockIdx.x, ctas);
+  const uint64_t u1 = att_first_unit(sc.total, blockIdx.x + 1, ctas);
+  att_find(w, sc, u0);
+
+  // ---- the stream of 64-key tiles: a cursor that runs ahead of the work
+  struct Cursor {
+    uint32_t b, hr, tile;
+    AttWork::Seq s;
+  };
+  Cursor in;
+  in.b = sc.seq;
+  in.s = w.seq(in.b);
+  {
+    const uint64_t rel = u0 - sc.before;
+    in.hr = static_cast<uint32_t>(rel / in.s.tiles);
+    in.tile = static_cast<uint32_t>(rel - static_cast<uint64_t>(in.hr) * in.s.tiles);
+  }
+  Cursor at = in;
+  auto advance = [&](Cursor& c) {
+    if (++c.tile < c.s.tiles) return;
+    c.tile = 0;
+    if (++c.hr < c.s.row_tiles * w.kv.n_kv) return;
+    c.hr = 0;
+    do {
+      ++c.b;
+      c.s = w.seq(c.b);
+    } while (c.s.tiles == 0);
+  };
+  // the lane's position (16 per warp) in the cache: byte offset, -1 if none
+  auto lookup = [&](const Cursor& c) -> int64_t {
+    const int i = static_cast<int>(c.tile * kAttKeys) + 16 * warp + (lane & 15);
+    if (i >= c.s.keys) return -1;
+    return w.kv.offset(c.b, c.hr / c.s.row_tiles, static_cast<uint32_t>(c.s.key(i)));
+  };
+  const uint32_t ring = smem_u32(smem) + warp * (kAttStages * L::kStage);
+  constexpr int CPR = L::kRow / 16;  // 16-byte chunks of a row
+  constexpr int RPI = 32 / CPR;      // rows of one instruction
+  auto issue = [&](int slot, int64_t off) {
+    const uint32_t dst = ring + slot * L::kStage;
+    const int col = lane % CPR;
+#pragma unroll
+    for (int i = 0; i < 16 / RPI; ++i) {
+      const int row = RPI * i + lane / CPR;
+      const int64_t o = __shfl_sync(0xffffffffu, off, row);
+      const uint32_t d = dst + row * L::kRow + ((col ^ (row & 7)) << 4);
+      const int64_t a = o < 0 ? 0 : o + 16 * col;
+      cp_async_16(d, w.kv.k + a, o < 0 ? 0 : 16);
+      cp_async_16(d + 16 * L::kRow, w.kv.v + a, o < 0 ? 0 : 16);
+    }
+  };
+
+  const uint64_t n = u1 - u0;
+  uint64_t ahead = 0;  // units issued
+  uint32_t masks[kAttStages];
+  int64_t off = lookup(in);
+#pragma unroll
+  for (int i = 0; i < kAttStages - 1; ++i) {
+    masks[i] = 0;
+    if (ahead < n) {
+      masks[i] = __ballot_sync(0xffffffffu, off >= 0) & 0xffffu;
+      issue(i, off);
+      if (++ahead < n) {
+        advance(in);
+        off = lookup(in);
+      }
+    }
+    cp_async_commit();
+  }
+  masks[kAttStages - 1] = 0;
+
+  // ---- the rows of the current row tile
+  uint32_t qf[NT][KS][2];
+  float m[NT][2], l[NT][2], o[NT][KS][4];
+  int prow[NT][2];  // MULTI: position of the lane's rows, -1 for none
+  auto begin_rows = [&]() {
+    const uint32_t hk = at.hr / at.s.row_tiles;
+    const uint32_t r0 = (at.hr - hk * at.s.row_tiles) * NR;
+    const uint32_t rows = static_cast<uint32_t>(at.s.count) * w.group;
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      const uint32_t r = r0 + 8 * x + g;
+      const uint32_t tok = w.by_group.div(r);
+      const bool have = r < rows;
+      const T* src = reinterpret_cast<const T*>(
+          q + (have ? (at.s.first + tok) * ld_q +
+                          static_cast<int64_t>(hk * w.group + r - tok * w.group) * (2 * D)
+                    : 0));
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        qf[x][s][0] = have ? *reinterpret_cast<const uint32_t*>(src + 16 * s + 2 * t4) : 0u;
+        qf[x][s][1] = have ? *reinterpret_cast<const uint32_t*>(src + 16 * s + 8 + 2 * t4) : 0u;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[x][s][c] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        m[x][c] = -INFINITY;
+        l[x][c] = 0.f;
+        if constexpr (MULTI) {
+          const uint32_t rr = r0 + 8 * x + 2 * t4 + c;
+          prow[x][c] = rr < rows ? at.s.len - at.s.count + static_cast<int>(w.by_group.div(rr)) : -1;
+        }
+      }
+    }
+  };
+  begin_rows();
+  uint32_t tile0 = at.tile;
+
+  // ldmatrix addresses: lane L gives row L & 7 of matrix L >> 3
+  const int mi = lane >> 3, mr = lane & 7;
+  const uint32_t k_row = ((mi & 1) * 8 + mr) * L::kRow, v_row = ((mi >> 1) * 8 + mr) * L::kRow;
+
+  int slot = 0;
+  for (uint64_t u = 0; u < n; ++u) {
+    cp_async_wait<kAttStages - 2>();
+    __syncwarp();
+    {
+      // refill the slot that the previous tile left
+      const int fill = slot == 0 ? kAttStages - 1 : slot - 1;
+      uint32_t mk = 0;
+      if (ahead < n) {
+        mk = __ballot_sync(0xffffffffu, off >= 0) & 0xffffu;
+        issue(fill, off);
+        if (++ahead < n) {
+          advance(in);
+          off = lookup(in);
+        }
+      }
+      cp_async_commit();
+#pragma unroll
+      for (int i = 0; i < kAttStages; ++i)
+        if (i == fill) masks[i] = mk;
+    }
+    uint32_t mask = masks[0];
+#pragma unroll
+    for (int i = 1; i < kAttStages; ++i)
+      if (i == slot) mask = masks[i];
+    const uint32_t kb = ring + slot * L::kStage, vb = kb + 16 * L::kRow;
+
+    // S^T = K Q^T: lane holds keys g and g + 8 of rows 2 t4, 2 t4 + 1
+    float s[NT][4];
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[x][c] = 0.f;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      uint32_t a0, a1, a2, a3;
+      ldmatrix_x4(kb + k_row + (((2 * i + (mi >> 1)) ^ mr) << 4), a0, a1, a2, a3);
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+        mma_16816<DT == kBF16>(s[x], a0, a1, a2, a3, qf[x][i][0], qf[x][i][1]);
+    }
+    const bool in0 = (mask >> g) & 1, in1 = (mask >> (g + 8)) & 1;
+    uint32_t pb[NT][2];
+    bool moved = false;
+    float corr[NT][2];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      float v[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        bool see = c < 2 ? in0 : in1;
+        if constexpr (MULTI) {
+          const int key = at.s.key(static_cast<int>(at.tile * kAttKeys) + 16 * warp + g + (c < 2 ? 0 : 8));
+          const int p = prow[x][c & 1];
+          see = see && key <= p && (w.window == 0 || key > p - w.window || key < w.sinks);
+        }
+        v[c] = see ? s[x][c] * scale_log2 : -INFINITY;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float top = fmaxf(v[c], v[c + 2]);
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float mn = fmaxf(m[x][c], top);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        corr[x][c] = exp2_approx(m[x][c] - base);
+        moved |= mn != m[x][c];
+        m[x][c] = mn;
+        v[c] = exp2_approx(v[c] - base);
+        v[c + 2] = exp2_approx(v[c + 2] - base);
+        l[x][c] = l[x][c] * corr[x][c] + v[c] + v[c + 2];
+      }
+      // weights of the second product in the operand type, keys along k
+      pb[x][0] = movmatrix_trans(pack2<DT>(v[0], v[1]));
+      pb[x][1] = movmatrix_trans(pack2<DT>(v[2], v[3]));
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[x][i][c] *= corr[x][c & 1];
+    }
+    // O^T += V^T P^T: lane holds dimensions 16 i + g, + 8 of its two rows
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      uint32_t a0, a1, a2, a3;
+      ldmatrix_x4_trans(vb + v_row + (((2 * i + (mi & 1)) ^ mr) << 4), a0, a1, a2, a3);
+#pragma unroll
+      for (int x = 0; x < NT; ++x) mma_16816<DT == kBF16>(o[x][i], a0, a1, a2, a3, pb[x][0], pb[x][1]);
+    }
+    __syncwarp();
+    if (++slot == kAttStages) slot = 0;
+
+    if (u + 1 < n && at.tile + 1 < at.s.tiles) {
+      ++at.tile;
+      continue;
+    }
+    // ---- the row tile's keys in this CTA end here: join the four warps
+    const bool whole = tile0 == 0 && at.tile + 1 == at.s.tiles;
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], d);
+        if (g == 0) {
+          s_m[warp][8 * x + 2 * t4 + c] = m[x][c];
+          s_l[warp][8 * x + 2 * t4 + c] = l[x][c];
+        }
+      }
+    __syncthreads();
+    float* merge = reinterpret_cast<float*>(smem + L::kRing);
+    const uint32_t hk = at.hr / at.s.row_tiles;
+    const uint32_t r0 = (at.hr - hk * at.s.row_tiles) * NR;
+    const int rows = min(NR, static_cast<int>(at.s.count * w.group - r0));
+    float* part = att_slot<D, NR>(ws, 2 * blockIdx.x + (u < at.tile - tile0 + 1 ? 0 : 1));
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int r = 8 * x + 2 * t4 + c;
+        float top = s_m[0][r];
+#pragma unroll
+        for (int i = 1; i < kAttWarps; ++i) top = fmaxf(top, s_m[i][r]);
+        const float f = exp2_approx(m[x][c] - (top == -INFINITY ? 0.f : top));
+        float* dst = merge + (warp * 8 + 2 * t4 + c) * L::kPad;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          dst[16 * i + g] = o[x][i][c] * f;
+          dst[16 * i + g + 8] = o[x][i][c + 2] * f;
+        }
+      }
+      __syncthreads();
+      for (int e = threadIdx.x; e < 8 * D; e += 32 * kAttWarps) {
+        const int r = 8 * x + e / D, c = e % D;
+        if (r >= rows) break;
+        float top = s_m[0][r], sum = 0.f, v = 0.f;
+#pragma unroll
+        for (int i = 1; i < kAttWarps; ++i) top = fmaxf(top, s_m[i][r]);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < kAttWarps; ++i) {
+          sum += s_l[i][r] * exp2_approx(s_m[i][r] - base);
+          v += merge[(i * 8 + e / D) * L::kPad + c];
+        }
+        if (whole) {
+          const uint32_t tok = w.by_group.div(r0 + r);
+          T* dst = reinterpret_cast<T*>(out + (at.s.first + tok) * ld_o +
+                                        static_cast<int64_t>(hk * w.group + r0 + r - tok * w.group) * (2 * D));
+          dst[c] = DType<DT>::from_f32(sum != 0.f ? v / sum : 0.f);
+        } else {
+          part[2 * NR + r * D + c] = v;
+          if (c == 0) {
+            part[r] = top;
+            part[NR + r] = sum;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (u + 1 < n) {
+      advance(at);
+      tile0 = 0;
+      begin_rows();
+    }
+  }
+  cp_async_wait<0>();
+}
+
+// Joins the parts of each row tile whose keys were split. One CTA per row
+// (blockIdx.x = row of kv head's row tiles, blockIdx.y = sequence, in strides):
+// the parts' factors first, then their outputs, a thread per dimension.
+template <int DT, int D, int NR>
+__global__ void __launch_bounds__(32 * kAttWarps)
+    attention_join_kernel(char* out, const AttWork w, int64_t ld_o, uint32_t launched,
+                          const float* __restrict__ ws) {
+  using T = typename DType<DT>::T;
+  constexpr int kThreads = 32 * kAttWarps, kSets = kThreads / D;
+  __shared__ AttScan sc;
+  __shared__ float s_f[kAttMaxCtas], s_red[kAttWarps], s_v[kThreads];
+  // The lengths are older than the first kernel, which let this one start.
+  att_scan(w, sc);
+  const uint64_t total = sc.total;
+  const uint32_t ctas = att_ctas(total, launched);
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t per = (w.kv.batch + kThreads - 1) / kThreads;
+  for (uint32_t b = blockIdx.y; b < w.kv.batch; b += gridDim.y) {
+    const AttWork::Seq s = w.seq(b);
+    if (s.tiles < 2) continue;
+    uint64_t before = sc.part[b / per];
+    for (uint32_t i = b / per * per; i < b; ++i) before += w.units(w.seq(i));
+    for (uint32_t x = blockIdx.x; x < s.row_tiles * w.kv.n_kv * NR; x += gridDim.x) {
+      const uint32_t hr = x / NR, r = x % NR;
+      const uint32_t hk = hr / s.row_tiles, row = (hr - hk * s.row_tiles) * NR + r;
+      if (row >= s.count * w.group) continue;
+      const uint64_t f = before + static_cast<uint64_t>(hr) * s.tiles, e = f + s.tiles - 1;
+      auto owner = [&](uint64_t u) {
+        uint32_t c = static_cast<uint32_t>(u * ctas / total);
+        while (att_first_unit(total, c + 1, ctas) <= u) ++c;
+        return c;
+      };
+      const uint32_t c0 = owner(f), parts = owner(e) - c0 + 1;
+      if (parts == 1) continue;  // written whole by its CTA
+      const bool late = att_first_unit(total, c0, ctas) != f;  // the first part is its CTA's second
+      auto slot = [&](uint32_t i) {
+        return ws + static_cast<size_t>(2 * (c0 + i) + (i == 0 && late)) * NR * (D + 2);
+      };
+      float top = -INFINITY;
+      for (uint32_t i = threadIdx.x; i < parts; i += kThreads) {
+        const float m = slot(i)[r];
+        s_f[i] = m;
+        top = fmaxf(top, m);
+      }
+      top = block_reduce<true>(top, s_red);
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+      for (uint32_t i = threadIdx.x; i < parts; i += kThreads) {
+        const float k = exp2_approx(s_f[i] - base);
+        s_f[i] = k;
+        sum += slot(i)[NR + r] * k;
+      }
+      sum = block_reduce<false>(sum, s_red);  // (its barriers publish s_f too)
+      const int c = threadIdx.x % D;
+      float v = 0.f;
+#pragma unroll 8
+      for (uint32_t i = threadIdx.x / D; i < parts; i += kSets)
+        v += slot(i)[2 * NR + r * D + c] * s_f[i];
+      if constexpr (kSets > 1) {
+        s_v[threadIdx.x] = v;
+        __syncthreads();
+        for (int k = 1; k < kSets; ++k) v += s_v[(threadIdx.x + k * D) % kThreads];
+      }
+      if (threadIdx.x < D) {
+        const uint32_t tok = w.by_group.div(row);
+        T* dst = reinterpret_cast<T*>(out + (s.first + tok) * ld_o +
+                                      static_cast<int64_t>(hk * w.group + row - tok * w.group) * (2 * D));
+        dst[c] = DType<DT>::from_f32(sum != 0.f ? v / sum : 0.f);
+      }
+      __syncthreads();  // s_f and s_v are written again
+    }
+  }
+}
+
+// Most units that a call can have, from what the host knows (the table's width).
+inline uint64_t att_most_units(size_t batch, size_t tokens, size_t group, size_t n_kv, size_t keys,
+                               size_t nr, bool multi) {
+  const uint64_t tiles = std::max<uint64_t>(1, (keys + kAttKeys - 1) / kAttKeys);
+  const uint64_t row_tiles = multi ? std::min<uint64_t>(tokens * group, (tokens * group) / nr + batch)
+                                   : batch * ((group + nr - 1) / nr);
+  return tiles * row_tiles * n_kv;
+}
+
+template <typename K>
+inline cudaError_t launch_pdl(K kern, dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                              void** args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kern), args);
+}
+
+// Dynamic shared memory past 48 KB has to be asked for once per device.
+template <typename K>
+inline cudaError_t allow_smem(K kern, int smem, int device, uint64_t* done) {
+  if (device < 64 && (*done >> device & 1)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && device < 64) *done |= 1ull << device;
+  return e;
+}
+
+template <int DT, int D, int NT, bool MULTI>
+cudaError_t launch_attention_split_t(const AttentionProblem& p, const PagedView& kv) {
+  static uint64_t done = 0;  // a lost update only repeats the call
+  auto kern = attention_split_kernel<DT, D, NT, MULTI>;
+  cudaError_t e = allow_smem(kern, AttLayout<D>::kSmem, p.device, &done);
+  if (e != cudaSuccess) return e;
+  AttWork w;
+  w.kv = kv;
+  w.tokens = static_cast<uint32_t>(p.tokens);
+  w.group = static_cast<uint32_t>(p.n_q / kv.n_kv);
+  w.row_tile = 8 * NT;
+  w.by_group = FastDiv(w.group);
+  w.window = p.window;
+  w.sinks = p.sinks;
+  const size_t keys = static_cast<size_t>(kv.width) * kv.page.d;
+  const uint64_t most = att_most_units(kv.batch, p.tokens, w.group, kv.n_kv, keys, 8 * NT, MULTI);
+  uint32_t ctas = static_cast<uint32_t>(
+      std::min<uint64_t>(most, std::min(2 * p.sm_count, kAttMaxCtas)));
+  const char* q = static_cast<const char*>(p.q);
+  char* out = static_cast<char*>(p.out);
+  int64_t ld_q = static_cast<int64_t>(p.ld_q) * 2, ld_o = static_cast<int64_t>(p.ld_out) * 2;
+  float sl = p.scale * 1.4426950408889634f;
+  float* ws = static_cast<float*>(p.workspace);
+  void* a[] = {&q, &out, &w, &ld_q, &ld_o, &sl, &ws};
+  e = launch_pdl(kern, dim3(ctas), 32 * kAttWarps, AttLayout<D>::kSmem, p.stream, a);
+  // no row tile can be split: its keys fit one unit
+  if (e != cudaSuccess || keys <= kAttKeys || ctas == 1) return e;
+  const uint64_t rows = static_cast<uint64_t>(kv.n_kv) * 8 * NT *
+                        ((w.group * (MULTI ? (p.tokens + kv.batch - 1) / kv.batch : 1) + 8 * NT - 1) / (8 * NT));
+  const float* cws = ws;
+  void* b[] = {&out, &w, &ld_o, &ctas, &cws};
+  return launch_pdl(attention_join_kernel<DT, D, 8 * NT>,
+                    dim3(static_cast<uint32_t>(std::min<uint64_t>(rows, 4096)),
+                         std::min<uint32_t>(kv.batch, 65535)),
+                    32 * kAttWarps, 0, p.stream, b);
+}
+
+inline size_t att_row_tile(size_t group, bool multi) { return multi || group > 8 ? 16 : 8; }
+
+inline size_t attention_split_workspace(size_t batch, size_t tokens, size_t group, size_t n_kv,
+                                        size_t keys, size_t d, bool multi) {
+  const size_t nr = att_row_tile(group, multi);
+  const uint64_t most = att_most_units(batch, tokens, group, n_kv, keys, nr, multi);
+  return std::min<uint64_t>(most, kAttMaxCtas) * 2 * nr * (d + 2) * sizeof(float);
+}
+
+cudaError_t launch_attention_split(const AttentionProblem& p, const PagedView& kv) {
+  const bool multi = kv.q_start != nullptr;
+  const bool two = att_row_tile(p.n_q / kv.n_kv, multi) == 16;
+#define CAWQ_ATT(DT, D)                                                    \
+  (multi ? launch_attention_split_t<DT, D, 2, true>(p, kv)                 \
+         : two ? launch_attention_split_t<DT, D, 2, false>(p, kv)          \
+               : launch_attention_split_t<DT, D, 1, false>(p, kv))
+  if (p.dtype == kF16) return p.d == 64 ? CAWQ_ATT(kF16, 64) : CAWQ_ATT(kF16, 128);
+  return p.d == 64 ? CAWQ_ATT(kBF16, 64) : CAWQ_ATT(kBF16, 128);
 #undef CAWQ_ATT
-  return cudaGetLastError();
 }
 
 }  // namespace cawq

@@ -36,7 +36,7 @@ struct AttentionProblem {
   int window, sinks;
   int dtype;
   void* workspace;
-  int sm_count;
+  int sm_count, device;
   cudaStream_t stream;
 };
 
@@ -99,6 +99,8 @@ static cawq_status check_paged(const cawq_paged_kv* kv, size_t tokens, size_t n_
       kv->page_size > kMaxInt || kv->table_width > kMaxInt / kv->page_size)
     return fail(CAWQ_ERR_INVALID_SHAPE,
                 "pages, batch, tokens and table_width * page_size must be below 2^31");
+  if (tokens > kMaxInt / (n_q / kv->n_kv))
+    return fail(CAWQ_ERR_INVALID_SHAPE, "tokens * n_q / n_kv must be below 2^31");
   if (kv->stride_page % 8 != 0 || kv->stride_head % 8 != 0 || kv->stride_token % 8 != 0)
     return fail(CAWQ_ERR_ALIGNMENT, "cache strides must be multiples of 8 elements");
   if (kv->ld_table < kv->table_width)
@@ -167,8 +169,8 @@ static cawq_status attention(const void* q, void* out, const cawq_paged_kv* kv, 
   const AttentionProblem p = {q, out, tokens, n_q, kv->head_dim, ld_q, ld_out, scale,
                               static_cast<int>(std::min(window, kMaxInt)),
                               static_cast<int>(std::min(sinks, kMaxInt)), dtype, workspace,
-                              dev.sm_count, static_cast<cudaStream_t>(stream)};
-  const cudaError_t e = launch_attention(p, paged_view(*kv, 2, decode));
+                              dev.sm_count, dev.device, static_cast<cudaStream_t>(stream)};
+  const cudaError_t e = launch_attention_split(p, paged_view(*kv, 2, decode));
   return e == cudaSuccess ? CAWQ_OK : cuda_fail(e, "attention launch");
 }
 
@@ -221,10 +223,10 @@ CAWQ_API cawq_status cawq_rope_append(const void* q, const void* k, const void* 
 }
 
 CAWQ_API size_t cawq_attention_workspace(const cawq_paged_kv* kv, size_t tokens, size_t n_q) {
-  (void)kv;
-  (void)tokens;
-  (void)n_q;
-  return 0;
+  if (!kv || kv->n_kv == 0 || tokens == 0) return 0;
+  return attention_split_workspace(kv->batch, tokens, n_q / kv->n_kv, kv->n_kv,
+                                   kv->table_width * kv->page_size, kv->head_dim,
+                                   kv->q_start != nullptr);
 }
 
 CAWQ_API cawq_status cawq_attention_decode(const void* q, void* out, const cawq_paged_kv* kv,
