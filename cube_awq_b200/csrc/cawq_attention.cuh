@@ -37,6 +37,12 @@ namespace cawq {
 constexpr int kAttWarps = 4;
 constexpr int kAttKeys = 16 * kAttWarps;  // keys of a unit
 constexpr int kAttStages = 3;
+// Units that a row tile counts for beside its key tiles: beginning and ending
+// one (rows of q, the join of the warps, the output) takes a CTA about as long
+// as streaming two tiles. Without it a batch of many short sequences and a few
+// long ones left the CTAs with the short ones last (64 sequences of 1 to 8000
+// tokens, 28 / 4 heads: 62 us).
+constexpr uint32_t kAttRowCost = 2;
 constexpr int kAttMaxCtas = 320;  // most CTAs of a launch (two per SM)
 
 template <int D>
@@ -98,7 +104,7 @@ struct AttWork {
 
   // Sequence b: its rows, its keys in order of position without the hidden
   // ones between the sinks and the window of its first new token, and its
-  // units (64-key tiles x kv heads x row tiles). A sequence with new tokens
+  // units: kv heads x row tiles x (kAttRowCost, then 64-key tiles). A sequence with new tokens
   // and no keys has one tile per row tile all the same: its rows are zeros.
   struct Seq {
     int first, count, len, start, head, keys;
@@ -118,7 +124,7 @@ struct AttWork {
     return s;
   }
   __device__ __forceinline__ uint64_t units(const Seq& s) const {
-    return static_cast<uint64_t>(s.tiles) * s.row_tiles * kv.n_kv;
+    return s.tiles ? static_cast<uint64_t>(s.tiles + kAttRowCost) * s.row_tiles * kv.n_kv : 0;
   }
 };
 
@@ -176,7 +182,7 @@ __device__ __forceinline__ void att_find(const AttWork& w, AttScan& sc, uint64_t
   __syncthreads();
 }
 
-// CTA c of n works on units [first(c), first(c + 1)); n is at most the number
+// CTA c of n works on the key tiles among units [first(c), first(c + 1)); n is at most the number
 // of units, so that no CTA between two of a row tile's is without a part.
 __device__ __forceinline__ uint32_t att_ctas(uint64_t total, uint32_t launched) {
   return static_cast<uint32_t>(min(total, static_cast<uint64_t>(launched)));
@@ -202,7 +208,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
   constexpr int NR = 8 * NT, KS = D / 16;
   extern __shared__ __align__(128) uint8_t smem[];
   AttScan& sc = *reinterpret_cast<AttScan*>(smem + L::kRing);  // read before the first merge
-  __shared__ float s_m[kAttWarps][NR], s_l[kAttWarps][NR];
+  __shared__ float s_m[kAttWarps][NR], s_f[kAttWarps][NR], s_top[NR];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
 
@@ -220,17 +226,20 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
     uint32_t b, hr, tile;
     AttWork::Seq s;
   };
+  int64_t left = static_cast<int64_t>(u1 - u0);  // units not issued yet
   Cursor in;
   in.b = sc.seq;
   in.s = w.seq(in.b);
   {
     const uint64_t rel = u0 - sc.before;
-    in.hr = static_cast<uint32_t>(rel / in.s.tiles);
-    in.tile = static_cast<uint32_t>(rel - static_cast<uint64_t>(in.hr) * in.s.tiles);
+    in.hr = static_cast<uint32_t>(rel / (in.s.tiles + kAttRowCost));
+    const uint32_t r = static_cast<uint32_t>(rel - static_cast<uint64_t>(in.hr) * (in.s.tiles + kAttRowCost));
+    in.tile = r < kAttRowCost ? 0 : r - kAttRowCost;
+    left -= r < kAttRowCost ? kAttRowCost - r : 0;
   }
+  if (left <= 0) return;  // nothing but the cost of a row tile that the next CTA begins
   Cursor at = in;
-  auto advance = [&](Cursor& c) {
-    if (++c.tile < c.s.tiles) return;
+  auto next_rows = [&](Cursor& c) {
     c.tile = 0;
     if (++c.hr < c.s.row_tiles * w.kv.n_kv) return;
     c.hr = 0;
@@ -238,6 +247,15 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
       ++c.b;
       c.s = w.seq(c.b);
     } while (c.s.tiles == 0);
+  };
+  // one tile on, while there are units; false past the CTA's last tile
+  auto advance = [&](Cursor& c, int64_t& units) -> bool {
+    --units;
+    if (++c.tile < c.s.tiles) return units > 0;
+    units -= kAttRowCost;
+    if (units <= 0) return false;
+    next_rows(c);
+    return true;
   };
   // the lane's position (16 per warp) in the cache: byte offset, -1 if none
   auto lookup = [&](const Cursor& c) -> int64_t {
@@ -262,61 +280,72 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
     }
   };
 
-  const uint64_t n = u1 - u0;
-  uint64_t ahead = 0;  // units issued
+  int64_t todo = left;  // units not worked off yet
+  bool more = true;     // `in` stands on a tile of this CTA's
   uint32_t masks[kAttStages];
   int64_t off = lookup(in);
-#pragma unroll
-  for (int i = 0; i < kAttStages - 1; ++i) {
-    masks[i] = 0;
-    if (ahead < n) {
-      masks[i] = __ballot_sync(0xffffffffu, off >= 0) & 0xffffu;
-      issue(i, off);
-      if (++ahead < n) {
-        advance(in);
-        off = lookup(in);
-      }
+  auto refill = [&](int slot) -> uint32_t {
+    uint32_t mask = 0;
+    if (more) {
+      mask = __ballot_sync(0xffffffffu, off >= 0) & 0xffffu;
+      issue(slot, off);
+      more = advance(in, left);
+      if (more) off = lookup(in);
     }
     cp_async_commit();
-  }
+    return mask;
+  };
+#pragma unroll
+  for (int i = 0; i < kAttStages - 1; ++i) masks[i] = refill(i);
   masks[kAttStages - 1] = 0;
 
   // ---- the rows of the current row tile
   uint32_t qf[NT][KS][2];
   float m[NT][2], l[NT][2], o[NT][KS][4];
   int prow[NT][2];  // MULTI: position of the lane's rows, -1 for none
-  auto begin_rows = [&]() {
-    const uint32_t hk = at.hr / at.s.row_tiles;
-    const uint32_t r0 = (at.hr - hk * at.s.row_tiles) * NR;
-    const uint32_t rows = static_cast<uint32_t>(at.s.count) * w.group;
+  auto load_rows = [&](const Cursor& c) {
+    const uint32_t hk = c.hr / c.s.row_tiles;
+    const uint32_t r0 = (c.hr - hk * c.s.row_tiles) * NR;
+    const uint32_t rows = static_cast<uint32_t>(c.s.count) * w.group;
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
       const uint32_t r = r0 + 8 * x + g;
       const uint32_t tok = w.by_group.div(r);
       const bool have = r < rows;
       const T* src = reinterpret_cast<const T*>(
-          q + (have ? (at.s.first + tok) * ld_q +
+          q + (have ? (c.s.first + tok) * ld_q +
                           static_cast<int64_t>(hk * w.group + r - tok * w.group) * (2 * D)
                     : 0));
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         qf[x][s][0] = have ? *reinterpret_cast<const uint32_t*>(src + 16 * s + 2 * t4) : 0u;
         qf[x][s][1] = have ? *reinterpret_cast<const uint32_t*>(src + 16 * s + 8 + 2 * t4) : 0u;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[x][s][c] = 0.f;
       }
+      if constexpr (MULTI) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        m[x][c] = -INFINITY;
-        l[x][c] = 0.f;
-        if constexpr (MULTI) {
-          const uint32_t rr = r0 + 8 * x + 2 * t4 + c;
-          prow[x][c] = rr < rows ? at.s.len - at.s.count + static_cast<int>(w.by_group.div(rr)) : -1;
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t rr = r0 + 8 * x + 2 * t4 + k;
+          prow[x][k] = rr < rows ? c.s.len - c.s.count + static_cast<int>(w.by_group.div(rr)) : -1;
         }
       }
     }
   };
-  begin_rows();
+  auto clear = [&]() {
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[x][s][c] = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        m[x][c] = -INFINITY;
+        l[x][c] = 0.f;
+      }
+    }
+  };
+  load_rows(at);
+  clear();
   uint32_t tile0 = at.tile;
 
   // ldmatrix addresses: lane L gives row L & 7 of matrix L >> 3
@@ -324,22 +353,13 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
   const uint32_t k_row = ((mi & 1) * 8 + mr) * L::kRow, v_row = ((mi >> 1) * 8 + mr) * L::kRow;
 
   int slot = 0;
-  for (uint64_t u = 0; u < n; ++u) {
+  for (bool first_rows = true;;) {
     cp_async_wait<kAttStages - 2>();
     __syncwarp();
     {
       // refill the slot that the previous tile left
       const int fill = slot == 0 ? kAttStages - 1 : slot - 1;
-      uint32_t mk = 0;
-      if (ahead < n) {
-        mk = __ballot_sync(0xffffffffu, off >= 0) & 0xffffu;
-        issue(fill, off);
-        if (++ahead < n) {
-          advance(in);
-          off = lookup(in);
-        }
-      }
-      cp_async_commit();
+      const uint32_t mk = refill(fill);
 #pragma unroll
       for (int i = 0; i < kAttStages; ++i)
         if (i == fill) masks[i] = mk;
@@ -418,29 +438,26 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
     __syncwarp();
     if (++slot == kAttStages) slot = 0;
 
-    if (u + 1 < n && at.tile + 1 < at.s.tiles) {
-      ++at.tile;
-      continue;
-    }
+    const Cursor done = at;
+    const bool go_on = advance(at, todo);
+    if (go_on && at.tile != 0) continue;
     // ---- the row tile's keys in this CTA end here: join the four warps
-    const bool whole = tile0 == 0 && at.tile + 1 == at.s.tiles;
+    const bool whole = tile0 == 0 && done.tile + 1 == done.s.tiles;
+    if (go_on) load_rows(at);  // of the next one, while this one ends
 #pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], d);
-        if (g == 0) {
-          s_m[warp][8 * x + 2 * t4 + c] = m[x][c];
-          s_l[warp][8 * x + 2 * t4 + c] = l[x][c];
-        }
+        if (g == 0) s_m[warp][8 * x + 2 * t4 + c] = m[x][c];
       }
     __syncthreads();
     float* merge = reinterpret_cast<float*>(smem + L::kRing);
-    const uint32_t hk = at.hr / at.s.row_tiles;
-    const uint32_t r0 = (at.hr - hk * at.s.row_tiles) * NR;
-    const int rows = min(NR, static_cast<int>(at.s.count * w.group - r0));
-    float* part = att_slot<D, NR>(ws, 2 * blockIdx.x + (u < at.tile - tile0 + 1 ? 0 : 1));
+    const uint32_t hk = done.hr / done.s.row_tiles;
+    const uint32_t r0 = (done.hr - hk * done.s.row_tiles) * NR;
+    const int rows = min(NR, static_cast<int>(done.s.count * w.group - r0));
+    float* part = att_slot<D, NR>(ws, 2 * blockIdx.x + (first_rows ? 0 : 1));
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
 #pragma unroll
@@ -450,6 +467,10 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
 #pragma unroll
         for (int i = 1; i < kAttWarps; ++i) top = fmaxf(top, s_m[i][r]);
         const float f = exp2_approx(m[x][c] - (top == -INFINITY ? 0.f : top));
+        if (g == 0) {  // this warp's sum on the common scale
+          s_f[warp][r] = l[x][c] * f;
+          if (warp == 0) s_top[r] = top;
+        }
         float* dst = merge + (warp * 8 + 2 * t4 + c) * L::kPad;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
@@ -461,35 +482,31 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
       for (int e = threadIdx.x; e < 8 * D; e += 32 * kAttWarps) {
         const int r = 8 * x + e / D, c = e % D;
         if (r >= rows) break;
-        float top = s_m[0][r], sum = 0.f, v = 0.f;
-#pragma unroll
-        for (int i = 1; i < kAttWarps; ++i) top = fmaxf(top, s_m[i][r]);
-        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, v = 0.f;
 #pragma unroll
         for (int i = 0; i < kAttWarps; ++i) {
-          sum += s_l[i][r] * exp2_approx(s_m[i][r] - base);
+          sum += s_f[i][r];
           v += merge[(i * 8 + e / D) * L::kPad + c];
         }
         if (whole) {
           const uint32_t tok = w.by_group.div(r0 + r);
-          T* dst = reinterpret_cast<T*>(out + (at.s.first + tok) * ld_o +
+          T* dst = reinterpret_cast<T*>(out + (done.s.first + tok) * ld_o +
                                         static_cast<int64_t>(hk * w.group + r0 + r - tok * w.group) * (2 * D));
           dst[c] = DType<DT>::from_f32(sum != 0.f ? v / sum : 0.f);
         } else {
           part[2 * NR + r * D + c] = v;
           if (c == 0) {
-            part[r] = top;
+            part[r] = s_top[r];
             part[NR + r] = sum;
           }
         }
       }
       __syncthreads();
     }
-    if (u + 1 < n) {
-      advance(at);
-      tile0 = 0;
-      begin_rows();
-    }
+    if (!go_on) break;
+    first_rows = false;
+    tile0 = 0;
+    clear();
   }
   cp_async_wait<0>();
 }
@@ -521,7 +538,9 @@ __global__ void __launch_bounds__(32 * kAttWarps)
       const uint32_t hr = x / NR, r = x % NR;
       const uint32_t hk = hr / s.row_tiles, row = (hr - hk * s.row_tiles) * NR + r;
       if (row >= s.count * w.group) continue;
-      const uint64_t f = before + static_cast<uint64_t>(hr) * s.tiles, e = f + s.tiles - 1;
+      // units of its first and its last key tile
+      const uint64_t f = before + static_cast<uint64_t>(hr) * (s.tiles + kAttRowCost) + kAttRowCost;
+      const uint64_t e = f + s.tiles - 1;
       auto owner = [&](uint64_t u) {
         uint32_t c = static_cast<uint32_t>(u * ctas / total);
         while (att_first_unit(total, c + 1, ctas) <= u) ++c;
@@ -529,7 +548,8 @@ __global__ void __launch_bounds__(32 * kAttWarps)
       };
       const uint32_t c0 = owner(f), parts = owner(e) - c0 + 1;
       if (parts == 1) continue;  // written whole by its CTA
-      const bool late = att_first_unit(total, c0, ctas) != f;  // the first part is its CTA's second
+      // whether that CTA worked on another row tile before
+      const bool late = att_first_unit(total, c0, ctas) < f - kAttRowCost;
       auto slot = [&](uint32_t i) {
         return ws + static_cast<size_t>(2 * (c0 + i) + (i == 0 && late)) * NR * (D + 2);
       };
@@ -572,7 +592,7 @@ __global__ void __launch_bounds__(32 * kAttWarps)
 // Most units that a call can have, from what the host knows (the table's width).
 inline uint64_t att_most_units(size_t batch, size_t tokens, size_t group, size_t n_kv, size_t keys,
                                size_t nr, bool multi) {
-  const uint64_t tiles = std::max<uint64_t>(1, (keys + kAttKeys - 1) / kAttKeys);
+  const uint64_t tiles = std::max<uint64_t>(1, (keys + kAttKeys - 1) / kAttKeys) + kAttRowCost;
   const uint64_t row_tiles = multi ? std::min<uint64_t>(tokens * group, (tokens * group) / nr + batch)
                                    : batch * ((group + nr - 1) / nr);
   return tiles * row_tiles * n_kv;
