@@ -101,6 +101,7 @@ struct AttWork {
   uint32_t tokens, group, row_tile;  // group = n_q / n_kv, row_tile = NR
   FastDiv by_group;
   int window, sinks;
+  uint32_t most_rows;  // sequences with more rows belong to the tile kernel
 
   // Sequence b: its rows, its keys in order of position without the hidden
   // ones between the sinks and the window of its first new token, and its
@@ -120,7 +121,9 @@ struct AttWork {
     s.head = min(sinks, s.start);
     s.keys = s.len - s.start + s.head;
     s.row_tiles = (static_cast<uint32_t>(s.count) * group + row_tile - 1) / row_tile;
-    s.tiles = s.count > 0 ? max(1, (s.keys + kAttKeys - 1) / kAttKeys) : 0u;
+    s.tiles = s.count > 0 && s.count * group <= most_rows
+                  ? max(1, (s.keys + kAttKeys - 1) / kAttKeys)
+                  : 0u;
     return s;
   }
   __device__ __forceinline__ uint64_t units(const Seq& s) const {
@@ -589,6 +592,22 @@ __global__ void __launch_bounds__(32 * kAttWarps)
   }
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+
+inline AttWork att_work(const AttentionProblem& p, const PagedView& kv, uint32_t row_tile,
+                        uint32_t most_rows = 0xffffffffu) {
+  AttWork w;
+  w.kv = kv;
+  w.tokens = static_cast<uint32_t>(p.tokens);
+  w.group = static_cast<uint32_t>(p.n_q / kv.n_kv);
+  w.row_tile = row_tile;
+  w.by_group = FastDiv(w.group);
+  w.window = p.window;
+  w.sinks = p.sinks;
+  w.most_rows = most_rows;
+  return w;
+}
+
 // Most units that a call can have, from what the host knows (the table's width).
 inline uint64_t att_most_units(size_t batch, size_t tokens, size_t group, size_t n_kv, size_t keys,
                                size_t nr, bool multi) {
@@ -625,19 +644,13 @@ inline cudaError_t allow_smem(K kern, int smem, int device, uint64_t* done) {
 }
 
 template <int DT, int D, int NT, bool MULTI>
-cudaError_t launch_attention_split_t(const AttentionProblem& p, const PagedView& kv) {
+cudaError_t launch_attention_split_t(const AttentionProblem& p, const PagedView& kv,
+                                     uint32_t most_rows) {
   static uint64_t done = 0;  // a lost update only repeats the call
   auto kern = attention_split_kernel<DT, D, NT, MULTI>;
   cudaError_t e = allow_smem(kern, AttLayout<D>::kSmem, p.device, &done);
   if (e != cudaSuccess) return e;
-  AttWork w;
-  w.kv = kv;
-  w.tokens = static_cast<uint32_t>(p.tokens);
-  w.group = static_cast<uint32_t>(p.n_q / kv.n_kv);
-  w.row_tile = 8 * NT;
-  w.by_group = FastDiv(w.group);
-  w.window = p.window;
-  w.sinks = p.sinks;
+  AttWork w = att_work(p, kv, 8 * NT, most_rows);
   const size_t keys = static_cast<size_t>(kv.width) * kv.page.d;
   const uint64_t most = att_most_units(kv.batch, p.tokens, w.group, kv.n_kv, keys, 8 * NT, MULTI);
   uint32_t ctas = static_cast<uint32_t>(
@@ -645,7 +658,7 @@ cudaError_t launch_attention_split_t(const AttentionProblem& p, const PagedView&
   const char* q = static_cast<const char*>(p.q);
   char* out = static_cast<char*>(p.out);
   int64_t ld_q = static_cast<int64_t>(p.ld_q) * 2, ld_o = static_cast<int64_t>(p.ld_out) * 2;
-  float sl = p.scale * 1.4426950408889634f;
+  float sl = p.scale * kLog2e;
   float* ws = static_cast<float*>(p.workspace);
   void* a[] = {&q, &out, &w, &ld_q, &ld_o, &sl, &ws};
   e = launch_pdl(kern, dim3(ctas), 32 * kAttWarps, AttLayout<D>::kSmem, p.stream, a);
@@ -670,13 +683,14 @@ inline size_t attention_split_workspace(size_t batch, size_t tokens, size_t grou
   return std::min<uint64_t>(most, kAttMaxCtas) * 2 * nr * (d + 2) * sizeof(float);
 }
 
-cudaError_t launch_attention_split(const AttentionProblem& p, const PagedView& kv) {
+cudaError_t launch_attention_split(const AttentionProblem& p, const PagedView& kv,
+                                   uint32_t most_rows = 0xffffffffu) {
   const bool multi = kv.q_start != nullptr;
   const bool two = att_row_tile(p.n_q / kv.n_kv, multi) == 16;
 #define CAWQ_ATT(DT, D)                                                    \
-  (multi ? launch_attention_split_t<DT, D, 2, true>(p, kv)                 \
-         : two ? launch_attention_split_t<DT, D, 2, false>(p, kv)          \
-               : launch_attention_split_t<DT, D, 1, false>(p, kv))
+  (multi ? launch_attention_split_t<DT, D, 2, true>(p, kv, most_rows)                 \
+         : two ? launch_attention_split_t<DT, D, 2, false>(p, kv, most_rows)          \
+               : launch_attention_split_t<DT, D, 1, false>(p, kv, most_rows))
   if (p.dtype == kF16) return p.d == 64 ? CAWQ_ATT(kF16, 64) : CAWQ_ATT(kF16, 128);
   return p.d == 64 ? CAWQ_ATT(kBF16, 64) : CAWQ_ATT(kBF16, 128);
 #undef CAWQ_ATT

@@ -1,0 +1,514 @@
+// cawq_attention_tile.cuh — attention of many query rows over a paged cache on
+// the 5th-generation tensor cores (sm_100a): prompts and chunks of prompts.
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c (q . k_j) - m),  c = scale log2(e)
+//
+// over the visible positions j of the row. Bound by the tensor cores: 4 D
+// operations per (row, visible key).
+//
+// A CTA takes 256 query rows of one (sequence, kv head), as two halves of 128:
+// the rows are the G = n_q / n_kv query heads of consecutive tokens, token by
+// token, so the heads that share keys share their loads whatever G is, and the
+// key blocks of 128 that the causal mask or the window cut are few. Warps:
+//   0-3, 4-7  softmax of half 0 and 1, one row a thread
+//   8         tensor memory, one thread issues every MMA
+//   9         the producer: K_j and V_j of block j through one ring of
+//             128-key stages (TMA, 128-byte swizzle; one box per page, or per
+//             power of two that divides the page)
+//   10, 11    idle
+// Tensor memory: S_0, S_1 (128 fp32 columns each), O_0, O_1 (D each). The
+// issuing thread's order is S_0(0) S_1(0), then per block PV_0(j) S_0(j + 1)
+// PV_1(j) S_1(j + 1): while the softmax of one half works, the tensor cores do
+// the other half's products. The weights P, rounded to the operand type, go
+// back into tensor memory over the S they came from and are the A operand of
+// PV; V, which lies key by key, is its MN-major B operand.
+//
+// The running maximum m moves only when a row's block maximum exceeds it by
+// more than 2^8: p stays below 2^8 either way, nothing overflows (the sums are
+// fp32, f16 holds 65504), and the row's O is rescaled a few times per row
+// instead of once per block. MMAs complete in order, so when S(j) is there,
+// PV(j - 1) has been added to O and the softmax warps may rescale it.
+//
+// Stale memory. Pages that no row of the tile needs (past the end, before the
+// window) are not read: their boxes are requested outside the tensor and
+// arrive as zeros. The last page's rows past the end may hold anything; for K
+// they only reach masked scores, for V the box is written row by row with
+// zeros past the end, since 0 * NaN is NaN. A page number outside the cache
+// hides its keys (s_bad) and sets the error bit.
+//
+// Every wait is bounded (2 s); on a timeout the kernel sets bit 0 of the
+// device error word, stops issuing, waits (bounded) for what it issued, frees
+// its TMEM and returns.
+#pragma once
+
+#include "cawq_attention.cuh"
+#include "cawq_tcgen05.cuh"
+
+namespace cawq {
+
+constexpr int kTileRows = 256;
+constexpr int kTileKeys = 128;
+constexpr int kTileThreads = 384;
+constexpr float kTileSlack = 8.f;  // log2 of how far a row's maximum may be exceeded
+
+template <int D>
+struct TileLayout {
+  static constexpr int kHalf = 128 * D * 2;  // 128 rows of q, or keys, or values
+  static constexpr int kBlk = 128 * 128;     // their 64-element column block
+  static constexpr int kStages = D == 128 ? 5 : 10;
+  static constexpr int kOffKV = 2 * kHalf;
+  static constexpr int kOffBars = kOffKV + kStages * kHalf;
+  static constexpr int kSmem = 1024 + kOffBars + 512;
+};
+
+struct TileArgs {
+  const char* q;
+  char* out;
+  AttWork w;
+  int64_t ld_q, ld_o;
+  float scale_log2;   // > 0
+  uint32_t flip;      // 0x80008000 with a negative scale: q's signs turn
+  uint32_t least;     // sequences with fewer rows belong to the split kernel
+  uint32_t box;       // keys of a TMA box: divides page size and 128, a multiple of 8
+};
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    attention_tile_kernel(const __grid_constant__ CUtensorMap tm_k,
+                          const __grid_constant__ CUtensorMap tm_v,
+                          const __grid_constant__ TileArgs a) {
+  using L = TileLayout<D>;
+  constexpr int NS = L::kStages, CB = D / 64;
+  constexpr uint32_t kTmemCols = 512;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBars);
+  uint64_t* empty = full + NS;
+  uint64_t* q_full = empty + NS;
+  uint64_t* s_full = q_full + 1;  // [2]
+  uint64_t* p_full = s_full + 2;  // [2]
+  uint64_t* o_full = p_full + 2;  // [2]
+  uint64_t* drain = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  __shared__ uint32_t s_bad[8], s_sum[kTileThreads / 32], s_seq, s_tile;
+  const AttWork& w = a.w;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  pdl_wait();
+  pdl_launch_dependents();
+  // ---- which tile: the sequences' tiles in order, a sequence's last tile first
+  // (the later a causal tile, the longer it takes)
+  const uint32_t index = blockIdx.x / w.kv.n_kv, hk = blockIdx.x - index * w.kv.n_kv;
+  {
+    auto tiles = [&](uint32_t b) -> uint32_t {
+      int first, count;
+      w.kv.rows(b, w.tokens, &first, &count);
+      const uint32_t rows = static_cast<uint32_t>(count) * w.group;
+      return rows >= a.least ? (rows + kTileRows - 1) / kTileRows : 0u;
+    };
+    const uint32_t per = (w.kv.batch + kTileThreads - 1) / kTileThreads;
+    const uint32_t b0 = min(w.kv.batch, tid * per), b1 = min(w.kv.batch, b0 + per);
+    uint32_t n = 0;
+    for (uint32_t b = b0; b < b1; ++b) n += tiles(b);
+    uint32_t inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) s_sum[warp] = inc;
+    if (tid == 0) s_seq = 0xffffffffu;
+    __syncthreads();
+    uint32_t at = inc - n;
+    for (int i = 0; i < warp; ++i) at += s_sum[i];
+    if (index >= at && index < at + n) {
+      uint32_t b = b0;
+      for (;; ++b) {
+        const uint32_t t = tiles(b);
+        if (index < at + t) {
+          s_tile = t - 1 - (index - at);
+          break;
+        }
+        at += t;
+      }
+      s_seq = b;
+    }
+    __syncthreads();
+  }
+  const uint32_t b = s_seq;
+  if (b == 0xffffffffu) return;  // the grid is sized for the most tiles there can be
+
+  // ---- the tile's rows and key blocks
+  int first, count;
+  w.kv.rows(b, w.tokens, &first, &count);
+  const int len = w.kv.len(b);
+  const uint32_t rows = static_cast<uint32_t>(count) * w.group;
+  const uint32_t p0 = s_tile * kTileRows;
+  const bool two = p0 + 128 < rows;
+  const int shift = len - count;  // position of the first new token
+  const int pos_lo = shift + static_cast<int>(w.by_group.div(p0));
+  const int pos_hi = shift + static_cast<int>(w.by_group.div(min(p0 + kTileRows, rows) - 1));
+  const int start = w.window > 0 ? max(0, pos_lo - w.window + 1) : 0;
+  const int head = (min(w.sinks, start) + kTileKeys - 1) / kTileKeys;  // blocks that hold sinks
+  const int main0 = max(start / kTileKeys, head);
+  const int nb = pos_hi < 0 ? 0 : head + max(0, pos_hi / kTileKeys - main0 + 1);
+  auto block_key = [&](int j) { return (j < head ? j : main0 + j - head) * kTileKeys; };
+
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(q_full, 256);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(drain, 1);
+    fence_mbarrier_init();
+    fence_proxy_async_smem();
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 8) tmem_alloc(tmem_slot, kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t sm = smem_u32(smem);
+
+  if (warp < 8) {
+    // ---------------------------------------------------------- softmax
+    const int half = warp >> 2;
+    // both halves' rows of q into shared memory, K-major with 128-byte swizzle
+    constexpr int CPR = D / 8;
+#pragma unroll 4
+    for (int i = tid; i < kTileRows * CPR; i += 256) {
+      const uint32_t r = i / CPR, c = i % CPR, p = p0 + r;
+      if (r >= 128 && !two) break;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (p < rows) {
+        const uint32_t tok = w.by_group.div(p);
+        v = *reinterpret_cast<const uint4*>(
+            a.q + (first + tok) * a.ld_q +
+            static_cast<int64_t>(hk * w.group + p - tok * w.group) * (2 * D) + 16 * c);
+        v.x ^= a.flip;
+        v.y ^= a.flip;
+        v.z ^= a.flip;
+        v.w ^= a.flip;
+      }
+      *reinterpret_cast<uint4*>(smem + (r >> 7) * L::kHalf + (c >> 3) * L::kBlk + (r & 127) * 128 +
+                                (((c & 7) ^ (r & 7)) << 4)) = v;
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(q_full);
+
+    if (half == 0 || two) {
+      const uint32_t p = p0 + tid;  // threads 0..255 are rows 0..255
+      const bool have = p < rows;
+      const uint32_t tok = have ? w.by_group.div(p) : 0u;
+      const int pos = shift + static_cast<int>(tok);
+      const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+      const uint32_t ts = tmem + lanes + 128 * half, to = tmem + lanes + 256 + 128 * half;
+      const float sl = a.scale_log2, slack = kTileSlack / sl;
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < nb; ++j) {
+        ok = mbar_wait_bounded(&s_full[half], j & 1);
+        ok = __all_sync(0xffffffffu, ok);  // tcgen05.ld / st are warp-collective
+        if (!ok) break;
+        tc_fence_after();
+        float s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32_nowait(ts + 32 * c, s[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_wait_ld(s[c]);
+        const int key0 = block_key(j);
+        const uint32_t bad = s_bad[j & 7];
+        const bool open = !have || (key0 + kTileKeys - 1 <= pos &&
+                                    (w.window == 0 || key0 > pos - w.window ||
+                                     key0 + kTileKeys - 1 < w.sinks));
+        if (bad != 0 || !__all_sync(0xffffffffu, open)) {
+          const int hi = pos - key0, lo = w.window > 0 ? pos - w.window + 1 - key0 : 0;
+          const int si = w.sinks - key0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const int x = 32 * c + k;
+              if (!(x <= hi && (x >= lo || x < si)) || (bad >> (x >> 3) & 1)) s[c][k] = -INFINITY;
+            }
+        }
+        float t[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          t[c] = s[c][0];
+#pragma unroll
+          for (int k = 1; k < 32; ++k) t[c] = fmaxf(t[c], s[c][k]);
+        }
+        const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        if (__any_sync(0xffffffffu, top > m + slack)) {
+          const float mn = fmaxf(m, top);
+          const float f = m == -INFINITY ? 0.f : exp2_approx((m - mn) * sl);
+          l *= f;
+          m = mn;
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              float o[16];
+              tmem_ld_32x32b_x16_nowait(to + 16 * c, o);
+              tmem_wait_ld(o);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] *= f;
+              tmem_st_32x32b_x16_nowait(to + 16 * c, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m * sl;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float pk[32];
+#pragma unroll
+          for (int k = 0; k < 64; k += 2) {
+            const float x = exp2_approx(fmaf(s[2 * h + (k >> 5)][k & 31], sl, -base));
+            const float y = exp2_approx(fmaf(s[2 * h + (k >> 5)][(k & 31) + 1], sl, -base));
+            sum[(k >> 1) & 3] += x + y;
+            pk[k >> 1] = __uint_as_float(pack2<DT>(x, y));
+          }
+          tmem_st_32x32b_x32_nowait(ts + 32 * h, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[half]);
+      }
+      if (ok && nb > 0) {
+        ok = mbar_wait_bounded(&o_full[half], 0);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      }
+      if (ok) {
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        char* dst = a.out + (first + tok) * a.ld_o +
+                    static_cast<int64_t>(hk * w.group + p - tok * w.group) * (2 * D);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          if (nb > 0) {
+            tmem_ld_32x32b_x32_nowait(to + 32 * c, o);
+            tmem_wait_ld(o);
+          }
+          if (!have) continue;
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (l != 0.f) {
+              v.x = pack2<DT>(o[k] * inv, o[k + 1] * inv);
+              v.y = pack2<DT>(o[k + 2] * inv, o[k + 3] * inv);
+              v.z = pack2<DT>(o[k + 4] * inv, o[k + 5] * inv);
+              v.w = pack2<DT>(o[k + 6] * inv, o[k + 7] * inv);
+            }
+            *reinterpret_cast<uint4*>(dst + 64 * c + 2 * k) = v;
+          }
+        }
+      }
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------- MMA issuer
+    if (lane == 0 && nb > 0) {
+      const uint32_t id_s = tw_idesc(DT == kBF16, kTileKeys);
+      constexpr uint32_t id_o = umma_idesc_f16(DT == kBF16, 128, D);
+      auto qk = [&](int h, int slot) {
+        const uint32_t qa = sm + h * L::kHalf, ka = sm + L::kOffKV + slot * L::kHalf;
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x) {
+          const uint32_t o = (x >> 2) * L::kBlk + 32 * (x & 3);
+          umma_f16(tmem + 128 * h, umma_desc_sw128(qa + o, 16, 1024),
+                   umma_desc_sw128(ka + o, 16, 1024), id_s, x > 0);
+        }
+        umma_commit(&s_full[h]);
+      };
+      auto pv = [&](int h, int slot, bool add) {
+        const uint32_t va = sm + L::kOffKV + slot * L::kHalf;
+#pragma unroll
+        for (int x = 0; x < kTileKeys / 16; ++x)
+          umma_f16_tmem_a(tmem + 256 + 128 * h, tmem + 128 * h + 8 * x,
+                          umma_desc_sw128(va + 2048 * x, L::kBlk, 1024), id_o, add || x > 0);
+      };
+      const int halves = two ? 2 : 1;
+      int slot = 0;
+      uint32_t par = 0;
+      auto next = [&]() {
+        if (++slot == NS) {
+          slot = 0;
+          par ^= 1u;
+        }
+      };
+      bool ok = mbar_wait_bounded(q_full, 0) && mbar_wait_bounded(&full[0], 0);
+      if (ok) {
+        tc_fence_after();
+        for (int h = 0; h < halves; ++h) qk(h, 0);
+        umma_commit(&empty[0]);
+        next();
+      }
+      for (int j = 0; j < nb && ok; ++j) {
+        const int sv = slot;
+        ok = mbar_wait_bounded(&full[sv], par);
+        next();
+        const int sk = slot;
+        const bool more = j + 1 < nb;
+        if (more) {
+          ok = ok && mbar_wait_bounded(&full[sk], par);
+          next();
+        }
+        for (int h = 0; h < halves && ok; ++h) {
+          ok = mbar_wait_bounded(&p_full[h], j & 1);
+          if (!ok) break;
+          tc_fence_after();
+          pv(h, sv, j > 0);
+          if (h + 1 == halves) umma_commit(&empty[sv]);
+          if (more) {
+            qk(h, sk);
+            if (h + 1 == halves) umma_commit(&empty[sk]);
+          } else {
+            umma_commit(&o_full[h]);
+          }
+        }
+      }
+      if (!ok) {
+        umma_commit(drain);
+        mbar_wait_bounded(drain, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // ------------------------------------------------- K / V producer
+    const uint32_t boxes = kTileKeys / a.box;
+    const uint32_t box_bytes = a.box * 128;  // of one 64-element column block
+    const int seen = min(len, pos_hi + 1);
+    int issued = 0;
+    bool ok = true;
+    for (int j = 0; j < nb && ok; ++j) {
+      const int key = block_key(j) + static_cast<int>(lane * a.box);  // this lane's box
+      const bool need = lane < boxes && key < seen &&
+                        (key + static_cast<int>(a.box) > start || key < min(w.sinks, start));
+      int page = -1, in_page = 0;
+      if (need) {
+        const uint32_t pg = w.kv.page.div(key);
+        page = w.kv.table[b * w.kv.ld_table + pg];
+        in_page = key - static_cast<int>(pg * w.kv.page.d);
+      }
+      const bool there = static_cast<uint32_t>(page) < w.kv.pages;
+      const uint32_t gone = __ballot_sync(0xffffffffu, need && !there);
+      if (gone != 0 && lane == 0) atomicOr(&g_cawq_device_error, kErrCache);
+      // the same by groups of 8 keys
+      const uint32_t bad = __ballot_sync(0xffffffffu, lane < 16 && (gone >> (8 * lane / a.box) & 1));
+      const bool cut = there && key + static_cast<int>(a.box) > len;  // ends inside the box
+      const uint32_t cuts = __ballot_sync(0xffffffffu, cut);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const int slot = issued % NS, use = issued / NS;
+        if (use > 0) ok = mbar_wait_bounded(&empty[slot], (use - 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t dst = L::kOffKV + slot * L::kHalf;
+        uint32_t bytes = L::kHalf;
+        if (kv == 1 && cuts != 0) {
+          // the values of the last page, with zeros past the sequence's end
+          const int from = __ffs(cuts) - 1;
+          const int pg = __shfl_sync(0xffffffffu, page, from);
+          const int ip = __shfl_sync(0xffffffffu, in_page, from);
+          const int left = len - __shfl_sync(0xffffffffu, key, from);
+          const char* src = w.kv.v + pg * w.kv.sp + hk * w.kv.sh + ip * w.kv.st;
+          for (uint32_t i = lane; i < a.box * (D / 8); i += 32) {
+            const uint32_t r = i / (D / 8), c = i % (D / 8), rr = from * a.box + r;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (static_cast<int>(r) < left)
+              v = *reinterpret_cast<const uint4*>(src + r * w.kv.st + 16 * c);
+            *reinterpret_cast<uint4*>(smem + dst + (c >> 3) * L::kBlk + rr * 128 +
+                                      (((c & 7) ^ (rr & 7)) << 4)) = v;
+          }
+          fence_proxy_async_smem();
+          bytes -= CB * box_bytes;
+        }
+        if (kv == 0 && lane == 0) s_bad[j & 7] = bad;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&full[slot], bytes);
+        __syncwarp();
+        if (lane < boxes && !(kv == 1 && cut)) {
+#pragma unroll
+          for (int h = 0; h < CB; ++h)
+            tma_load_4d(sm + dst + h * L::kBlk + lane * box_bytes, kv ? &tm_v : &tm_k, 64 * h,
+                        in_page, static_cast<int>(hk),
+                        there ? page : static_cast<int>(w.kv.pages), &full[slot]);
+        }
+        ++issued;
+      }
+    }
+    if (!ok)  // copies in flight end before the CTA does
+      for (int i = max(0, issued - NS); i < issued; ++i)
+        mbar_wait_bounded(&full[i % NS], (i / NS) & 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// The cache's keys or values as a 4-D tensor: elements, slots, heads, pages.
+inline bool encode_cache(CUtensorMap* map, int dtype, const void* base, const PagedView& kv,
+                         uint32_t d, uint32_t box) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  const uint64_t dims[4] = {d, kv.page.d, kv.n_kv, kv.pages};
+  // an extent of 1 never uses its stride, which may then be anything
+  const uint64_t strides[3] = {static_cast<uint64_t>(kv.page.d > 1 ? kv.st : 2 * d),
+                               static_cast<uint64_t>(kv.n_kv > 1 ? kv.sh : 2 * d),
+                               static_cast<uint64_t>(kv.pages > 1 ? kv.sp : 2 * d)};
+  const uint32_t bx[4] = {64, box, 1, 1}, es[4] = {1, 1, 1, 1};
+  return fn(map, dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+            4, const_cast<void*>(base), dims, strides, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == 0;
+}
+
+template <int DT, int D>
+cudaError_t launch_attention_tile_t(const AttentionProblem& p, const PagedView& kv, uint32_t least) {
+  static uint64_t done = 0;
+  auto kern = attention_tile_kernel<DT, D>;
+  cudaError_t e = allow_smem(kern, TileLayout<D>::kSmem, p.device, &done);
+  if (e != cudaSuccess) return e;
+  TileArgs a;
+  a.q = static_cast<const char*>(p.q);
+  a.out = static_cast<char*>(p.out);
+  a.w = att_work(p, kv, 0);
+  a.ld_q = static_cast<int64_t>(p.ld_q) * 2;
+  a.ld_o = static_cast<int64_t>(p.ld_out) * 2;
+  // scores of a scale of 0 are all equal: so they are at 1e-30
+  a.scale_log2 = std::max(std::abs(p.scale) * kLog2e, 1e-30f);
+  a.flip = p.scale < 0 ? 0x80008000u : 0u;
+  a.least = least;
+  a.box = 8;
+  while (a.box < kTileKeys && kv.page.d % (2 * a.box) == 0) a.box *= 2;
+  CUtensorMap mk, mv;
+  if (!encode_cache(&mk, DT, kv.k, kv, D, a.box) || !encode_cache(&mv, DT, kv.v, kv, D, a.box))
+    return cudaErrorInvalidValue;
+  const uint64_t tiles = p.tokens * a.w.group / kTileRows + std::min<uint64_t>(kv.batch, p.tokens);
+  void* args[] = {&mk, &mv, &a};
+  return launch_pdl(kern, dim3(static_cast<uint32_t>(tiles * kv.n_kv)), kTileThreads,
+                    TileLayout<D>::kSmem, p.stream, args);
+}
+
+cudaError_t launch_attention_tile(const AttentionProblem& p, const PagedView& kv, uint32_t least) {
+  if (p.dtype == kF16)
+    return p.d == 64 ? launch_attention_tile_t<kF16, 64>(p, kv, least)
+                     : launch_attention_tile_t<kF16, 128>(p, kv, least);
+  return p.d == 64 ? launch_attention_tile_t<kBF16, 64>(p, kv, least)
+                   : launch_attention_tile_t<kBF16, 128>(p, kv, least);
+}
+
+}  // namespace cawq

@@ -4,6 +4,7 @@
 // entry points (argument checks on the host; what only the device knows is
 // bounded in the kernels, see cawq_paged.cuh).
 #include <algorithm>
+#include <cmath>
 
 #include "cawq_common.cuh"
 
@@ -45,6 +46,7 @@ cudaError_t read_layer_error(uint32_t* word, int reset) { return read_own_error_
 }  // namespace cawq
 
 #include "cawq_attention.cuh"
+#include "cawq_attention_tile.cuh"
 #include "cawq_norm.cuh"
 #include "cawq_rope.cuh"
 
@@ -170,7 +172,13 @@ static cawq_status attention(const void* q, void* out, const cawq_paged_kv* kv, 
                               static_cast<int>(std::min(window, kMaxInt)),
                               static_cast<int>(std::min(sinks, kMaxInt)), dtype, workspace,
                               dev.sm_count, dev.device, static_cast<cudaStream_t>(stream)};
-  const cudaError_t e = launch_attention_split(p, paged_view(*kv, 2, decode));
+  const PagedView view = paged_view(*kv, 2, decode);
+  cudaError_t e;
+  if (decode || kv->pages == 0) {
+    e = launch_attention_split(p, view);
+  } else {
+    e = launch_attention_tile(p, view, 0);
+  }
   return e == cudaSuccess ? CAWQ_OK : cuda_fail(e, "attention launch");
 }
 

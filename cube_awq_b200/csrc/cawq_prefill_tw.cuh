@@ -67,6 +67,7 @@
 #pragma once
 
 #include "cawq_common.cuh"
+#include "cawq_tcgen05.cuh"
 
 namespace cawq {
 
@@ -113,24 +114,6 @@ struct TwLayout {
   }
 };
 
-// kind::f16 instruction descriptor with both operands K-major (A in TMEM,
-// B = X rows in shared memory), fp32 accumulate.
-__host__ __device__ constexpr uint32_t tw_idesc(bool bf16, uint32_t n) {
-  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((n >> 3) << 17) |
-         ((128u >> 4) << 24);
-}
-
-// D[tmem_d] (+)= A[tmem_a] · B[bdesc]: A from tensor memory.
-__device__ __forceinline__ void umma_f16_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
-                                                uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
 // 16 lanes x 256 bits, four times along the columns: lane t holds, per
 // repetition j, (lane t/4, column 8j + 2(t%4)), (same lane, + 1),
 // (lane t/4 + 8, column 8j + 2(t%4)), (same lane, + 1).
@@ -148,10 +131,6 @@ __device__ __forceinline__ void tmem_st_16x256b_x2(uint32_t taddr, const uint32_
   asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
                "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
-}
-
-__device__ __forceinline__ void tmem_wait_st() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 // 32 lanes x 16 consecutive fp32 columns -> 16 registers per thread.
