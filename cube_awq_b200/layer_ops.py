@@ -36,7 +36,13 @@ import torch
 
 from . import _lib
 from .errors import CubeAwqError, DTypeError, ShapeError, check
-from .kernel import _require_cuda, cawq_dtype, stream_handle
+from .kernel import _require_cuda, _torch_ext, cawq_dtype, stream_handle
+
+# Each operator first calls its compiled host path (csrc/cawq_torch.cpp), which
+# does the checks, the allocation and the C call in C++; it gives None for
+# arguments that do not fit (and an int where the C call failed), and the
+# functions here then say what is wrong. At decode sizes the host's work is of
+# the order of the kernels' own time.
 
 _SHAPE = _lib.CAWQ_ERR_INVALID_SHAPE
 _HALVES = (torch.float16, torch.bfloat16)
@@ -120,6 +126,13 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     None (it would be x). x, residual [..., d] f32, f16 or bf16, contiguous or
     2-D with a unit column stride. ``out`` may be x, ``residual_out`` may be
     ``residual`` (the residual stream updated in place)."""
+    ext = _torch_ext()
+    if ext is not None:
+        r = ext.rms_norm(x, weight, eps, residual, out, residual_out)
+        if r.__class__ is tuple:
+            return r
+        if r is not None:
+            check(r)
     return _norm(x, weight, eps, residual, out, x.dtype, residual_out, None)
 
 
@@ -132,6 +145,13 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     scales[...] = max |y| / 448 of a row (fp32), y8 = float8_e4m3fn(y / scale),
     the operands of an 8-bit product with row scales (a module that AutoAWQ
     left unquantised, such as lm_head)."""
+    ext = _torch_ext()
+    if ext is not None:
+        r = ext.rms_norm_fp8(x, weight, eps, residual, out, scales, residual_out)
+        if r.__class__ is tuple:
+            return r
+        if r is not None:
+            check(r)
     return _norm(x, weight, eps, residual, out, torch.float8_e4m3fn, residual_out, scales)
 
 
@@ -202,6 +222,13 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope: torch.T
     head turns with element i + head_dim / 2. ``out`` may be q itself. Without
     ``q_start`` there is one new token per sequence. A token of an empty slot
     (negative position) gets a zero q and is not stored."""
+    ext = _torch_ext()
+    if ext is not None:
+        r = ext.rope_append(q, k, v, rope, k_cache, v_cache, block_table, seq_lens, q_start, out)
+        if r.__class__ is torch.Tensor:
+            return r
+        if r is not None:
+            check(r)
     _same_device(q, k, v, rope, k_cache, v_cache, block_table, seq_lens, q_start, out)
     if q.dtype not in _HALVES:
         raise DTypeError("the rotary append takes f16 or bf16", _lib.CAWQ_ERR_DTYPE)
@@ -225,6 +252,14 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope: torch.T
 
 
 def _attention(q, k_cache, v_cache, block_table, seq_lens, q_start, scale, window, sinks, out):
+    ext = _torch_ext()
+    if ext is not None:
+        r = ext.attention(q, k_cache, v_cache, block_table, seq_lens, q_start, scale, window, sinks,
+                          out)
+        if r.__class__ is torch.Tensor:
+            return r
+        if r is not None:
+            check(r)
     _same_device(q, k_cache, v_cache, block_table, seq_lens, q_start, out)
     if q.dtype not in _HALVES:
         raise DTypeError("attention takes f16 or bf16", _lib.CAWQ_ERR_DTYPE)

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import cube_awq_b200 as cawq
+from cube_awq_b200.errors import CubeAwqError
 from layer_ref import FLOOR, ROUND, Cache, F32, assert_within, attention_ref, norm_ref, norm_rel
 
 pytestmark = pytest.mark.gpu
@@ -384,3 +385,23 @@ def test_empty_calls(cuda_device):
     assert cawq.attention_decode(q, c.k, c.v, table, none).shape == (0, 4, 128)
     zero = torch.zeros(2, dtype=torch.int32, device=cuda_device)
     assert cawq.attention_prefill(q, c.k, c.v, c.table, c.lens, zero).shape == (0, 4, 128)
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_both_host_paths(cuda_device, compiled, monkeypatch):
+    # the compiled host path, and the one in Python where it was not built
+    from cube_awq_b200 import layer_ops
+    if not compiled:
+        monkeypatch.setattr(layer_ops, "_torch_ext", lambda: None)
+    x, w = _randn((5, 640), BF16, cuda_device, 1), _randn((640,), BF16, cuda_device, 2)
+    y, h = cawq.rms_norm(x, w, 1e-6, residual=x)
+    _check_norm(x, w, 1e-6, x, y, h)
+    y8, s, h8 = cawq.rms_norm_fp8(x, w, 1e-6, residual=x)
+    assert torch.equal(h, h8) and y8.dtype == torch.float8_e4m3fn and s.shape == (5,)
+    _attend(cuda_device, BF16, [(1, 300), (1, 2)], 8, 2, 128, 16, 50, 3, decode=True)
+    _attend(cuda_device, BF16, [(30, 300), (2, 2)], 8, 2, 128, 16, 50, 3)
+    c, q, k, v, rope = _rope_case(cuda_device, F16, [(3, 40), (1, 1)], 4, 2, 64, 16, "pair")
+    out = cawq.rope_append(q, k, v, rope, c.k, c.v, c.table, c.lens, q_start=c.q_start)
+    assert out.shape == q.shape and torch.equal(c.v[int(c.table[1, 0]), :, 0], v[3])
+    with pytest.raises(CubeAwqError):
+        cawq.attention_decode(q[:2], c.k, c.v, c.table, c.lens, window=-1)
