@@ -617,32 +617,6 @@ inline uint64_t att_most_units(size_t batch, size_t tokens, size_t group, size_t
   return tiles * row_tiles * n_kv;
 }
 
-template <typename K>
-inline cudaError_t launch_pdl(K kern, dim3 grid, int threads, size_t smem, cudaStream_t stream,
-                              void** args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kern), args);
-}
-
-// Dynamic shared memory past 48 KB has to be asked for once per device.
-template <typename K>
-inline cudaError_t allow_smem(K kern, int smem, int device, uint64_t* done) {
-  if (device < 64 && (*done >> device & 1)) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess && device < 64) *done |= 1ull << device;
-  return e;
-}
-
 template <int DT, int D, int NT, bool MULTI>
 cudaError_t launch_attention_split_t(const AttentionProblem& p, const PagedView& kv,
                                      uint32_t most_rows) {

@@ -16,7 +16,7 @@ struct NormProblem {
   float* scales;  // non-null: y is e4m3
   size_t rows, d, ld_x, ld_res, ld_y, ld_res_out;
   float eps;
-  int dtype;
+  int dtype, sm_count;
   cudaStream_t stream;
 };
 
@@ -40,6 +40,34 @@ struct AttentionProblem {
   int sm_count, device;
   cudaStream_t stream;
 };
+
+// Launch with programmatic dependent launch: every kernel of this file begins
+// with griddepcontrol.wait.
+template <typename K>
+inline cudaError_t launch_pdl(K kern, dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                              void** args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kern), args);
+}
+
+// Dynamic shared memory past 48 KB has to be asked for once per device.
+template <typename K>
+inline cudaError_t allow_smem(K kern, int smem, int device, uint64_t* done) {
+  if (device < 64 && (*done >> device & 1)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && device < 64) *done |= 1ull << device;
+  return e;
+}
 
 cudaError_t read_layer_error(uint32_t* word, int reset) { return read_own_error_word(word, reset); }
 
@@ -80,7 +108,7 @@ static cawq_status rms_norm(const void* x, const void* weight, const void* resid
   cawq_status st = require_sm100(&dev);
   if (st != CAWQ_OK) return st;
   const NormProblem p = {x, weight, residual, y, residual_out, scales, rows, d, ld_x, ld_res,
-                         ld_y, ld_ro, eps, dtype, static_cast<cudaStream_t>(stream)};
+                         ld_y, ld_ro, eps, dtype, dev.sm_count, static_cast<cudaStream_t>(stream)};
   const cudaError_t e = launch_rms_norm(p);
   return e == cudaSuccess ? CAWQ_OK : cuda_fail(e, "RMS norm launch");
 }

@@ -7,28 +7,12 @@
 // the 8 that turn with them, so every access is 16 bytes.
 #pragma once
 
+#include "cawq_norm.cuh"
 #include "cawq_paged.cuh"
 
 namespace cawq {
 
-constexpr int kRopeThreads = 256;
-
-template <int DT>
-__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
-  using T = typename DType<DT>::T;
-  const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = DType<DT>::to_f32(e[i]);
-}
-template <int DT>
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  using T = typename DType<DT>::T;
-  uint4 u;
-  T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = DType<DT>::from_f32(f[i]);
-  return u;
-}
+constexpr int kRopeThreads = 1024;
 
 template <int DT>
 __global__ void __launch_bounds__(kRopeThreads)
@@ -36,26 +20,34 @@ __global__ void __launch_bounds__(kRopeThreads)
                        char* q_out, const PagedView kv, uint32_t tokens, uint32_t n_q, uint32_t d,
                        uint32_t rope_rows, int64_t ld_q, int64_t ld_k, int64_t ld_v,
                        int64_t ld_qo) {
+  using V = Vec16<DT>;
+  pdl_wait();
+  pdl_launch_dependents();
   const uint32_t t = blockIdx.x;
-  const uint32_t b = kv.sequence(t);
-  int pos = -1;
-  if (b < kv.batch) {
-    int first, count;
-    kv.rows(b, tokens, &first, &count);
-    pos = kv.len(b) - count + static_cast<int>(t) - first;
-  }
-  if (pos >= static_cast<int>(rope_rows)) {
-    atomicOr(&g_cawq_device_error, kErrCache);
-    pos = -1;
-  }
-  const uint32_t per = d / 16;  // threads a head takes
-  const uint32_t items = (n_q + 2 * kv.n_kv) * per;
+  const uint32_t shift = d == 64 ? 2 : 3;  // 4 or 8 threads a head
+  const uint32_t items = (n_q + 2 * kv.n_kv) << shift;
   const uint32_t half = d;  // bytes of half a head
-  for (uint32_t i = threadIdx.x; i < items; i += kRopeThreads) {
-    const uint32_t h = i / per, c = i - h * per;
+  int pos = -1;
+  uint32_t b = 0;
+  for (uint32_t i = threadIdx.x; i < items; i += blockDim.x) {
+    const uint32_t h = i >> shift, c = i & ((1u << shift) - 1);
     const char* src = h < n_q ? q + t * ld_q + (int64_t)h * 2 * d
                       : h < n_q + kv.n_kv ? k + t * ld_k + (int64_t)(h - n_q) * 2 * d
                                           : v + t * ld_v + (int64_t)(h - n_q - kv.n_kv) * 2 * d;
+    uint4 lo = *reinterpret_cast<const uint4*>(src + 16 * c);
+    uint4 hi = *reinterpret_cast<const uint4*>(src + half + 16 * c);
+    if (i == threadIdx.x) {  // once, while the first loads are under way
+      b = kv.sequence(t);
+      if (b < kv.batch) {
+        int first, count;
+        kv.rows(b, tokens, &first, &count);
+        pos = kv.len(b) - count + static_cast<int>(t) - first;
+      }
+      if (pos >= static_cast<int>(rope_rows)) {
+        atomicOr(&g_cawq_device_error, kErrCache);
+        pos = -1;
+      }
+    }
     char* dst;
     if (h < n_q) {
       dst = q_out + t * ld_qo + (int64_t)h * 2 * d;
@@ -66,22 +58,26 @@ __global__ void __launch_bounds__(kRopeThreads)
       if (at < 0) continue;
       dst = (is_v ? kv.v : kv.k) + at;
     }
-    uint4 lo = *reinterpret_cast<const uint4*>(src + 16 * c);
-    uint4 hi = *reinterpret_cast<const uint4*>(src + half + 16 * c);
     if (h < n_q + kv.n_kv) {
-      float a[8], e[8];
-      unpack8<DT>(lo, a);
-      unpack8<DT>(hi, e);
-      const float* cs = rope + (size_t)(pos < 0 ? 0 : pos) * d + 8 * c;
+      float a[8], e[8], cs[8], sn[8];
+      V::unpack(lo, a);
+      V::unpack(hi, e);
+      const float4* tab = reinterpret_cast<const float4*>(rope + (size_t)max(pos, 0) * d) + 2 * c;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4 x = pos < 0 ? make_float4(0, 0, 0, 0) : __ldg(tab + j);
+        const float4 y = pos < 0 ? make_float4(0, 0, 0, 0) : __ldg(tab + d / 8 + j);
+        cs[4 * j] = x.x, cs[4 * j + 1] = x.y, cs[4 * j + 2] = x.z, cs[4 * j + 3] = x.w;
+        sn[4 * j] = y.x, sn[4 * j + 1] = y.y, sn[4 * j + 2] = y.z, sn[4 * j + 3] = y.w;
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float x = pos < 0 ? 0.f : cs[j], y = pos < 0 ? 0.f : cs[d / 2 + j];
-        const float u = a[j] * x - e[j] * y, w = e[j] * x + a[j] * y;
-        a[j] = pos < 0 ? 0.f : u;
+        const float u = a[j] * cs[j] - e[j] * sn[j], w = e[j] * cs[j] + a[j] * sn[j];
+        a[j] = pos < 0 ? 0.f : u;  // a token of no place: zeros, whatever q holds
         e[j] = pos < 0 ? 0.f : w;
       }
-      lo = pack8<DT>(a);
-      hi = pack8<DT>(e);
+      lo = V::pack(a);
+      hi = V::pack(e);
     }
     *reinterpret_cast<uint4*>(dst + 16 * c) = lo;
     *reinterpret_cast<uint4*>(dst + half + 16 * c) = hi;
@@ -89,17 +85,22 @@ __global__ void __launch_bounds__(kRopeThreads)
 }
 
 cudaError_t launch_rope_append(const RopeProblem& p, const PagedView& kv) {
-  const dim3 grid(static_cast<uint32_t>(p.tokens));
-#define CAWQ_ROPE(DT)                                                                           \
-  rope_append_kernel<DT><<<grid, kRopeThreads, 0, p.stream>>>(                                 \
-      static_cast<const char*>(p.q), static_cast<const char*>(p.k),                            \
-      static_cast<const char*>(p.v), p.rope, static_cast<char*>(p.q_out), kv,                  \
-      static_cast<uint32_t>(p.tokens), static_cast<uint32_t>(p.n_q),                           \
-      static_cast<uint32_t>(p.d), static_cast<uint32_t>(p.rope_rows), (int64_t)p.ld_q * 2,     \
-      (int64_t)p.ld_k * 2, (int64_t)p.ld_v * 2, (int64_t)p.ld_q_out * 2)
-  if (p.dtype == kF16) CAWQ_ROPE(kF16); else CAWQ_ROPE(kBF16);
-#undef CAWQ_ROPE
-  return cudaGetLastError();
+  const char *q = static_cast<const char*>(p.q), *k = static_cast<const char*>(p.k);
+  const char* v = static_cast<const char*>(p.v);
+  const float* rope = p.rope;
+  char* q_out = static_cast<char*>(p.q_out);
+  PagedView view = kv;
+  uint32_t tokens = static_cast<uint32_t>(p.tokens), n_q = static_cast<uint32_t>(p.n_q);
+  uint32_t d = static_cast<uint32_t>(p.d), rope_rows = static_cast<uint32_t>(p.rope_rows);
+  int64_t ld_q = (int64_t)p.ld_q * 2, ld_k = (int64_t)p.ld_k * 2, ld_v = (int64_t)p.ld_v * 2;
+  int64_t ld_qo = (int64_t)p.ld_q_out * 2;
+  void* a[] = {&q, &k, &v, &rope, &q_out, &view, &tokens, &n_q, &d, &rope_rows, &ld_q, &ld_k,
+               &ld_v, &ld_qo};
+  // a thread per item where a CTA has room for a token's
+  const uint32_t items = (n_q + 2 * kv.n_kv) * (d / 16);
+  const int threads = static_cast<int>(std::min<uint32_t>((items + 31) / 32 * 32, kRopeThreads));
+  return launch_pdl(p.dtype == kF16 ? rope_append_kernel<kF16> : rope_append_kernel<kBF16>,
+                    dim3(tokens), threads, 0, p.stream, a);
 }
 
 }  // namespace cawq
