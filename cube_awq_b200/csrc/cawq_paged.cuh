@@ -55,15 +55,19 @@ struct PagedView {
     *first = a;
     *count = e - a;
   }
-  // the sequence of row t (batch if none) by bisection of q_start
+  // the sequence of row t (batch if none): how many q_start[b + 1] are <= t,
+  // by a search that a whole warp makes with 32 probes a step
   __device__ __forceinline__ uint32_t sequence(uint32_t t) const {
     if (!q_start) return t;
-    uint32_t lo = 0, hi = batch;  // the first b with q_start[b + 1] > t
-    while (lo < hi) {
-      const uint32_t mid = (lo + hi) >> 1;
-      if (q_start[mid + 1] > static_cast<int>(t)) hi = mid; else lo = mid + 1;
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t lo = 0, span = batch;
+    for (;;) {
+      const uint32_t step = (span + 31) / 32, at = lo + (lane + 1) * step - 1;
+      const bool past = (lane + 1) * step <= span && q_start[at + 1] <= static_cast<int>(t);
+      lo += __popc(__ballot_sync(0xffffffffu, past)) * step;
+      if (step <= 1) return lo;
+      span = min(step, batch - lo);
     }
-    return lo;
   }
   // byte offset of position j of sequence b, head h (the same in k and v);
   // -1 (and the error bit) if its page is none of the cache's. j < len(b).

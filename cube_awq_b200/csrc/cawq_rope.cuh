@@ -27,26 +27,37 @@ __global__ void __launch_bounds__(kRopeThreads)
   const uint32_t shift = d == 64 ? 2 : 3;  // 4 or 8 threads a head
   const uint32_t items = (n_q + 2 * kv.n_kv) << shift;
   const uint32_t half = d;  // bytes of half a head
+  auto source = [&](uint32_t i) {
+    const uint32_t h = i >> shift, c = i & ((1u << shift) - 1);
+    return (h < n_q ? q + t * ld_q + (int64_t)h * 2 * d
+                    : h < n_q + kv.n_kv ? k + t * ld_k + (int64_t)(h - n_q) * 2 * d
+                                        : v + t * ld_v + (int64_t)(h - n_q - kv.n_kv) * 2 * d) +
+           16 * c;
+  };
+  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+  if (threadIdx.x < items) {
+    const char* src = source(threadIdx.x);
+    lo = *reinterpret_cast<const uint4*>(src);
+    hi = *reinterpret_cast<const uint4*>(src + half);
+  }
+  // the position, while these loads are under way
+  const uint32_t b = kv.sequence(t);
   int pos = -1;
-  uint32_t b = 0;
+  if (b < kv.batch) {
+    int first, count;
+    kv.rows(b, tokens, &first, &count);
+    pos = kv.len(b) - count + static_cast<int>(t) - first;
+  }
+  if (pos >= static_cast<int>(rope_rows)) {
+    atomicOr(&g_cawq_device_error, kErrCache);
+    pos = -1;
+  }
   for (uint32_t i = threadIdx.x; i < items; i += blockDim.x) {
     const uint32_t h = i >> shift, c = i & ((1u << shift) - 1);
-    const char* src = h < n_q ? q + t * ld_q + (int64_t)h * 2 * d
-                      : h < n_q + kv.n_kv ? k + t * ld_k + (int64_t)(h - n_q) * 2 * d
-                                          : v + t * ld_v + (int64_t)(h - n_q - kv.n_kv) * 2 * d;
-    uint4 lo = *reinterpret_cast<const uint4*>(src + 16 * c);
-    uint4 hi = *reinterpret_cast<const uint4*>(src + half + 16 * c);
-    if (i == threadIdx.x) {  // once, while the first loads are under way
-      b = kv.sequence(t);
-      if (b < kv.batch) {
-        int first, count;
-        kv.rows(b, tokens, &first, &count);
-        pos = kv.len(b) - count + static_cast<int>(t) - first;
-      }
-      if (pos >= static_cast<int>(rope_rows)) {
-        atomicOr(&g_cawq_device_error, kErrCache);
-        pos = -1;
-      }
+    if (i != threadIdx.x) {
+      const char* src = source(i);
+      lo = *reinterpret_cast<const uint4*>(src);
+      hi = *reinterpret_cast<const uint4*>(src + half);
     }
     char* dst;
     if (h < n_q) {
