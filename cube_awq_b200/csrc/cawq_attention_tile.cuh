@@ -50,6 +50,7 @@ constexpr int kTileRows = 256;
 constexpr int kTileKeys = 128;
 constexpr int kTileThreads = 384;
 constexpr float kTileSlack = 8.f;  // log2 of how far a row's maximum may be exceeded
+constexpr int kTilePoly = 3;       // of 8 pairs of weights, how many take exp2_poly
 
 template <int D>
 struct TileLayout {
@@ -60,6 +61,72 @@ struct TileLayout {
   static constexpr int kOffBars = kOffKV + kStages * kHalf;
   static constexpr int kSmem = 1024 + kOffBars + 512;
 };
+
+// Two fp32 values in one register pair: sm_100's packed arithmetic.
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x of two values on the FMA pipe (the special-function unit alone takes as
+// long as the tensor cores here): Cody-Waite reduction x = n + f, |f| <= 1/2,
+// by adding and subtracting 1.5 * 2^23; 2^f by a polynomial that is minimax in
+// relative error on [-1/2, 1/2] (Remez exchange; 7.5e-5 of degree 3, enough
+// for weights that are rounded to bf16's 2^-9, 2.6e-6 of degree 4 for f16);
+// 2^n by adding n to the exponent. x <= 9; below -126 the result is no more
+// than 2^-126 (so also for -inf, where the other pairs get 0).
+template <int DT>
+__device__ __forceinline__ void exp2_poly(uint64_t x2, float& a, float& b) {
+  constexpr float kMagic = 12582912.f;
+  float x, y;
+  f2_unpack(x2, x, y);
+  x = fmaxf(x, -126.f);
+  y = fmaxf(y, -126.f);
+  x2 = f2_pack(x, y);
+  const uint64_t t = f2_add(x2, f2_pack(kMagic, kMagic));
+  const uint64_t n = f2_add(t, f2_pack(-kMagic, -kMagic));
+  const uint64_t f = f2_fma(n, f2_pack(-1.f, -1.f), x2);
+  uint64_t p;
+  if constexpr (DT == kBF16) {
+    p = f2_fma(f2_pack(0.05517167f, 0.05517167f), f, f2_pack(0.24261113f, 0.24261113f));
+    p = f2_fma(p, f, f2_pack(0.69326097f, 0.69326097f));
+    p = f2_fma(p, f, f2_pack(0.99992806f, 0.99992806f));
+  } else {
+    p = f2_fma(f2_pack(0.0095701022f, 0.0095701022f), f, f2_pack(0.055917859f, 0.055917859f));
+    p = f2_fma(p, f, f2_pack(0.24024744f, 0.24024744f));
+    p = f2_fma(p, f, f2_pack(0.69312179f, 0.69312179f));
+    p = f2_fma(p, f, f2_pack(0.99999928f, 0.99999928f));
+  }
+  float pa, pb, ta, tb;
+  f2_unpack(p, pa, pb);
+  f2_unpack(t, ta, tb);
+  a = __uint_as_float(__float_as_uint(pa) + (__float_as_uint(ta) << 23));
+  b = __uint_as_float(__float_as_uint(pb) + (__float_as_uint(tb) << 23));
+}
+
+// n ones from bit 0 on, for any n
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+}
 
 struct TileArgs {
   const char* q;
@@ -86,8 +153,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* empty = full + NS;
   uint64_t* q_full = empty + NS;
   uint64_t* s_full = q_full + 1;  // [2]
-  uint64_t* p_full = s_full + 2;  // [2]
-  uint64_t* o_full = p_full + 2;  // [2]
+  uint64_t* p_full = s_full + 2;  // [2][2]: halves of the rows, halves of the keys
+  uint64_t* o_full = p_full + 4;  // [2]
   uint64_t* drain = o_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   __shared__ uint32_t s_bad[8], s_sum[kTileThreads / 32], s_seq, s_tile;
@@ -162,7 +229,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     mbar_init(q_full, 256);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[2 * i], 128);
+      mbar_init(&p_full[2 * i + 1], 128);
       mbar_init(&o_full[i], 1);
     }
     mbar_init(drain, 1);
@@ -230,24 +298,31 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                     (w.window == 0 || key0 > pos - w.window ||
                                      key0 + kTileKeys - 1 < w.sinks));
         if (bad != 0 || !__all_sync(0xffffffffu, open)) {
-          const int hi = pos - key0, lo = w.window > 0 ? pos - w.window + 1 - key0 : 0;
+          // the row's visible keys as bits: up to its position, and in the
+          // window or among the sinks
+          const int hi = pos - key0 + 1, lo = w.window > 0 ? hi - w.window : 0;
           const int si = w.sinks - key0;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 4; ++c) {
+            uint32_t see = low_bits(hi - 32 * c) & (~low_bits(lo - 32 * c) | low_bits(si - 32 * c));
+            if (bad != 0) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const int x = 32 * c + k;
-              if (!(x <= hi && (x >= lo || x < si)) || (bad >> (x >> 3) & 1)) s[c][k] = -INFINITY;
+              for (int k = 0; k < 4; ++k)
+                if (bad >> (4 * c + k) & 1) see &= ~(0xffu << 8 * k);
             }
+#pragma unroll
+            for (int k = 0; k < 32; ++k) s[c][k] = see >> k & 1 ? s[c][k] : -INFINITY;
+          }
         }
         float t[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          t[c] = s[c][0];
+          t[c] = max3(s[c][0], s[c][1], s[c][2]);
 #pragma unroll
-          for (int k = 1; k < 32; ++k) t[c] = fmaxf(t[c], s[c][k]);
+          for (int k = 3; k < 31; k += 2) t[c] = max3(t[c], s[c][k], s[c][k + 1]);
+          t[c] = fmaxf(t[c], s[c][31]);
         }
-        const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        const float top = fmaxf(max3(t[0], t[1], t[2]), t[3]);
         if (__any_sync(0xffffffffu, top > m + slack)) {
           const float mn = fmaxf(m, top);
           const float f = m == -INFINITY ? 0.f : exp2_approx((m - mn) * sl);
@@ -266,23 +341,37 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
         }
         const float base = m == -INFINITY ? 0.f : m * sl;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t sl2 = f2_pack(sl, sl), nb2 = f2_pack(-base, -base);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float pk[32];
+        for (int c = 0; c < 4; ++c) {
+          float pk[16];
 #pragma unroll
-          for (int k = 0; k < 64; k += 2) {
-            const float x = exp2_approx(fmaf(s[2 * h + (k >> 5)][k & 31], sl, -base));
-            const float y = exp2_approx(fmaf(s[2 * h + (k >> 5)][(k & 31) + 1], sl, -base));
-            sum[(k >> 1) & 3] += x + y;
-            pk[k >> 1] = __uint_as_float(pack2<DT>(x, y));
+          for (int k = 0; k < 16; ++k) {
+            const uint64_t x2 = f2_fma(f2_pack(s[c][2 * k], s[c][2 * k + 1]), sl2, nb2);
+            float x, y;
+            if (k * kTilePoly % 8 < kTilePoly) {
+              exp2_poly<DT>(x2, x, y);
+            } else {
+              f2_unpack(x2, x, y);
+              x = exp2_approx(x);
+              y = exp2_approx(y);
+            }
+            sum[k & 1] = f2_add(sum[k & 1], f2_pack(x, y));
+            pk[k] = __uint_as_float(pack2<DT>(x, y));
           }
-          tmem_st_32x32b_x32_nowait(ts + 32 * h, pk);
+          tmem_st_32x32b_x16_nowait(ts + 16 * c, pk);
+          if (c & 1) {  // half of the keys' weights are there
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&p_full[2 * half + (c >> 1)]);
+          }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&p_full[half]);
+        {
+          float x, y;
+          f2_unpack(f2_add(sum[0], sum[1]), x, y);
+          l += x + y;
+        }
       }
       if (ok && nb > 0) {
         ok = mbar_wait_bounded(&o_full[half], 0);
@@ -290,7 +379,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tc_fence_after();
       }
       if (ok) {
-        const float inv = l != 0.f ? 1.f / l : 0.f;
+        const float inv = m != -INFINITY ? 1.f / l : 0.f;  // no key seen: zeros
         char* dst = a.out + (first + tok) * a.ld_o +
                     static_cast<int64_t>(hk * w.group + p - tok * w.group) * (2 * D);
 #pragma unroll
@@ -304,7 +393,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
           for (int k = 0; k < 32; k += 8) {
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (l != 0.f) {
+            if (m != -INFINITY) {
               v.x = pack2<DT>(o[k] * inv, o[k + 1] * inv);
               v.y = pack2<DT>(o[k + 2] * inv, o[k + 3] * inv);
               v.z = pack2<DT>(o[k + 4] * inv, o[k + 5] * inv);
@@ -330,10 +419,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         umma_commit(&s_full[h]);
       };
-      auto pv = [&](int h, int slot, bool add) {
+      auto pv = [&](int h, int slot, int part, bool add) {
         const uint32_t va = sm + L::kOffKV + slot * L::kHalf;
 #pragma unroll
-        for (int x = 0; x < kTileKeys / 16; ++x)
+        for (int x = 4 * part; x < 4 * part + 4; ++x)
           umma_f16_tmem_a(tmem + 256 + 128 * h, tmem + 128 * h + 8 * x,
                           umma_desc_sw128(va + 2048 * x, L::kBlk, 1024), id_o, add || x > 0);
       };
@@ -364,10 +453,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           next();
         }
         for (int h = 0; h < halves && ok; ++h) {
-          ok = mbar_wait_bounded(&p_full[h], j & 1);
+          ok = mbar_wait_bounded(&p_full[2 * h], j & 1);
           if (!ok) break;
           tc_fence_after();
-          pv(h, sv, j > 0);
+          pv(h, sv, 0, j > 0);
+          ok = mbar_wait_bounded(&p_full[2 * h + 1], j & 1);
+          if (!ok) break;
+          tc_fence_after();
+          pv(h, sv, 1, true);
           if (h + 1 == halves) umma_commit(&empty[sv]);
           if (more) {
             qk(h, sk);
