@@ -10,12 +10,13 @@
 // the rows are the G = n_q / n_kv query heads of consecutive tokens, token by
 // token, so the heads that share keys share their loads whatever G is, and the
 // key blocks of 128 that the causal mask or the window cut are few. Warps:
-//   0-3, 4-7  softmax of half 0 and 1, one row a thread
-//   8         tensor memory, one thread issues every MMA
-//   9         the producer: K_j and V_j of block j through one ring of
+//   0-7, 8-15 softmax of half 0 and 1: 16 rows a warp, four threads a row
+//             (with a row a thread and four warps a half a block took 2400
+//             cycles, most of them latency; the tensor cores need 1024)
+//   16        tensor memory, one thread issues every MMA
+//   17        the producer: K_j and V_j of block j through one ring of
 //             128-key stages (TMA, 128-byte swizzle; one box per page, or per
 //             power of two that divides the page)
-//   10, 11    idle
 // Tensor memory: S_0, S_1 (128 fp32 columns each), O_0, O_1 (D each). The
 // issuing thread's order is S_0(0) S_1(0), then per block PV_0(j) S_0(j + 1)
 // PV_1(j) S_1(j + 1): while the softmax of one half works, the tensor cores do
@@ -48,7 +49,7 @@ namespace cawq {
 
 constexpr int kTileRows = 256;
 constexpr int kTileKeys = 128;
-constexpr int kTileThreads = 384;
+constexpr int kTileThreads = 576;
 constexpr float kTileSlack = 8.f;  // log2 of how far a row's maximum may be exceeded
 constexpr int kTilePoly = 3;       // of 8 pairs of weights, how many take exp2_poly
 
@@ -123,6 +124,20 @@ __device__ __forceinline__ void exp2_poly(uint64_t x2, float& a, float& b) {
   b = __uint_as_float(__float_as_uint(pb) + (__float_as_uint(tb) << 23));
 }
 
+// 4 x 4 transpose among four neighbouring lanes: v[k] of lane t -> v[t] of lane k.
+__device__ __forceinline__ void quad_transpose(uint32_t (&v)[4], int t) {
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1) {  // exchange with lane t ^ d
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (k & d) continue;
+      const uint32_t give = t & d ? v[k] : v[k | d];
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, give, d);
+      if (t & d) v[k] = got; else v[k | d] = got;
+    }
+  }
+}
+
 // n ones from bit 0 on, for any n
 __device__ __forceinline__ uint32_t low_bits(int n) {
   return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
@@ -153,8 +168,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* empty = full + NS;
   uint64_t* q_full = empty + NS;
   uint64_t* s_full = q_full + 1;  // [2]
-  uint64_t* p_full = s_full + 2;  // [2][2]: halves of the rows, halves of the keys
-  uint64_t* o_full = p_full + 4;  // [2]
+  uint64_t* p_full = s_full + 2;  // [2]
+  uint64_t* o_full = p_full + 2;  // [2]
   uint64_t* drain = o_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   __shared__ uint32_t s_bad[8], s_sum[kTileThreads / 32], s_seq, s_tile;
@@ -226,11 +241,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(q_full, 256);
+    mbar_init(q_full, 512);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[2 * i], 128);
-      mbar_init(&p_full[2 * i + 1], 128);
+      mbar_init(&p_full[i], 256);
       mbar_init(&o_full[i], 1);
     }
     mbar_init(drain, 1);
@@ -239,20 +253,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  if (warp == 8) tmem_alloc(tmem_slot, kTmemCols);
+  if (warp == 16) tmem_alloc(tmem_slot, kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t sm = smem_u32(smem);
 
-  if (warp < 8) {
+  if (warp < 16) {
     // ---------------------------------------------------------- softmax
-    const int half = warp >> 2;
+    const int half = warp >> 3;
     // both halves' rows of q into shared memory, K-major with 128-byte swizzle
     constexpr int CPR = D / 8;
 #pragma unroll 4
-    for (int i = tid; i < kTileRows * CPR; i += 256) {
+    for (int i = tid; i < kTileRows * CPR; i += 512) {
       const uint32_t r = i / CPR, c = i % CPR, p = p0 + r;
       if (r >= 128 && !two) break;
       uint4 v = make_uint4(0, 0, 0, 0);
@@ -273,82 +287,121 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     mbar_arrive(q_full);
 
     if (half == 0 || two) {
-      const uint32_t p = p0 + tid;  // threads 0..255 are rows 0..255
-      const bool have = p < rows;
-      const uint32_t tok = have ? w.by_group.div(p) : 0u;
-      const int pos = shift + static_cast<int>(tok);
-      const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-      const uint32_t ts = tmem + lanes + 128 * half, to = tmem + lanes + 256 + 128 * half;
+      // this thread's rows r0 and r0 + 8 of the half, columns 8 j + 2 (lane % 4), + 1
+      const int t4 = lane & 3, r0 = 32 * (warp & 3) + 16 * ((warp >> 2) & 1) + (lane >> 2);
+      const uint32_t lanes = static_cast<uint32_t>(r0 & ~15) << 16;
+      const uint32_t ts = tmem + lanes + 128 * half;  // scores; the weights over their first half
+      const uint32_t to = tmem + lanes + 256 + 128 * half;
       const float sl = a.scale_log2, slack = kTileSlack / sl;
-      float m = -INFINITY, l = 0.f;
+      const uint64_t sl2 = f2_pack(sl, sl);
+      bool have[2];
+      int pos[2];
+      float m[2], l[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t p = p0 + 128 * half + r0 + 8 * i;
+        have[i] = p < rows;
+        pos[i] = shift + static_cast<int>(w.by_group.div(have[i] ? p : 0u));
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+      }
       bool ok = true;
       for (int j = 0; j < nb; ++j) {
         ok = mbar_wait_bounded(&s_full[half], j & 1);
         ok = __all_sync(0xffffffffu, ok);  // tcgen05.ld / st are warp-collective
         if (!ok) break;
         tc_fence_after();
-        float s[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32_nowait(ts + 32 * c, s[c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_wait_ld(s[c]);
+        float s[2][32];
+        tmem_ld_16x256b_x8_nowait(ts, s[0]);
+        tmem_ld_16x256b_x8_nowait(ts + 64, s[1]);
         const int key0 = block_key(j);
         const uint32_t bad = s_bad[j & 7];
-        const bool open = !have || (key0 + kTileKeys - 1 <= pos &&
-                                    (w.window == 0 || key0 > pos - w.window ||
-                                     key0 + kTileKeys - 1 < w.sinks));
-        if (bad != 0 || !__all_sync(0xffffffffu, open)) {
-          // the row's visible keys as bits: up to its position, and in the
-          // window or among the sinks
-          const int hi = pos - key0 + 1, lo = w.window > 0 ? hi - w.window : 0;
-          const int si = w.sinks - key0;
+        bool open = bad == 0;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t see = low_bits(hi - 32 * c) & (~low_bits(lo - 32 * c) | low_bits(si - 32 * c));
-            if (bad != 0) {
+        for (int i = 0; i < 2; ++i)
+          open = open && (!have[i] || (key0 + kTileKeys - 1 <= pos[i] &&
+                                       (w.window == 0 || key0 > pos[i] - w.window ||
+                                        key0 + kTileKeys - 1 < w.sinks)));
+        const bool cut = !__all_sync(0xffffffffu, open);
+        tmem_wait_ld(s[0]);
+        tmem_wait_ld(s[1]);
+        if (cut) {
+          // a row's visible keys as bits: up to its position, and in the window
+          // or among the sinks
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int hi = pos[i] - key0 + 1, lo = w.window > 0 ? hi - w.window : 0;
+            const int si = w.sinks - key0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t see =
+                  low_bits(hi - 32 * c) & (~low_bits(lo - 32 * c) | low_bits(si - 32 * c));
+              if (bad != 0) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  if (bad >> (4 * c + k) & 1) see &= ~(0xffu << 8 * k);
+              }
+              see >>= 2 * t4;
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                if (bad >> (4 * c + k) & 1) see &= ~(0xffu << 8 * k);
-            }
 #pragma unroll
-            for (int k = 0; k < 32; ++k) s[c][k] = see >> k & 1 ? s[c][k] : -INFINITY;
+                for (int e = 0; e < 2; ++e) {
+                  float& v = s[c >> 1][16 * (c & 1) + 4 * k + 2 * i + e];
+                  v = see >> (8 * k + e) & 1 ? v : -INFINITY;
+                }
+            }
           }
         }
-        float t[4];
+        float top[2];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          t[c] = max3(s[c][0], s[c][1], s[c][2]);
+        for (int i = 0; i < 2; ++i) {
+          float t[2];
 #pragma unroll
-          for (int k = 3; k < 31; k += 2) t[c] = max3(t[c], s[c][k], s[c][k + 1]);
-          t[c] = fmaxf(t[c], s[c][31]);
+          for (int c = 0; c < 2; ++c) {
+            t[c] = fmaxf(s[c][2 * i], s[c][2 * i + 1]);
+#pragma unroll
+            for (int k = 1; k < 8; ++k) t[c] = max3(t[c], s[c][4 * k + 2 * i], s[c][4 * k + 2 * i + 1]);
+          }
+          top[i] = fmaxf(t[0], t[1]);
         }
-        const float top = fmaxf(max3(t[0], t[1], t[2]), t[3]);
-        if (__any_sync(0xffffffffu, top > m + slack)) {
-          const float mn = fmaxf(m, top);
-          const float f = m == -INFINITY ? 0.f : exp2_approx((m - mn) * sl);
-          l *= f;
-          m = mn;
+#pragma unroll
+        for (int d = 1; d < 4; d <<= 1) {
+          top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
+          top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[0] + slack || top[1] > m[1] + slack)) {
+          float f[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float mn = fmaxf(m[i], top[i]);
+            f[i] = m[i] == -INFINITY ? 0.f : exp2_approx((m[i] - mn) * sl);
+            l[i] *= f[i];
+            m[i] = mn;
+          }
           if (j > 0) {
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
-              float o[16];
-              tmem_ld_32x32b_x16_nowait(to + 16 * c, o);
-              tmem_wait_ld(o);
+              float o[8];
+              tmem_ld_16x256b_x2(to + 16 * c, o);
 #pragma unroll
-              for (int k = 0; k < 16; ++k) o[k] *= f;
-              tmem_st_32x32b_x16_nowait(to + 16 * c, o);
+              for (int k = 0; k < 8; ++k) o[k] *= f[k >> 1 & 1];
+              tmem_st_16x256b_x2_nowait(to + 16 * c, o);
             }
           }
         }
-        const float base = m == -INFINITY ? 0.f : m * sl;
-        const uint64_t sl2 = f2_pack(sl, sl), nb2 = f2_pack(-base, -base);
-        uint64_t sum[2] = {0, 0};
+        uint64_t nb2[2], sum[2] = {0, 0};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float pk[16];
+        for (int i = 0; i < 2; ++i) {
+          const float base = m[i] == -INFINITY ? 0.f : m[i] * sl;
+          nb2[i] = f2_pack(-base, -base);
+        }
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const uint64_t x2 = f2_fma(f2_pack(s[c][2 * k], s[c][2 * k + 1]), sl2, nb2);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {  // repetition k / 2, row k % 2
+            const uint64_t x2 =
+                f2_fma(f2_pack(s[c][2 * k], s[c][2 * k + 1]), sl2, nb2[k & 1]);
             float x, y;
             if (k * kTilePoly % 8 < kTilePoly) {
               exp2_poly<DT>(x2, x, y);
@@ -358,20 +411,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               y = exp2_approx(y);
             }
             sum[k & 1] = f2_add(sum[k & 1], f2_pack(x, y));
-            pk[k] = __uint_as_float(pack2<DT>(x, y));
+            pk[k] = pack2<DT>(x, y);
           }
-          tmem_st_32x32b_x16_nowait(ts + 16 * c, pk);
-          if (c & 1) {  // half of the keys' weights are there
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&p_full[2 * half + (c >> 1)]);
-          }
+          tmem_st_16x128b_x8_nowait(ts + 32 * c, pk);
         }
-        {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
           float x, y;
-          f2_unpack(f2_add(sum[0], sum[1]), x, y);
-          l += x + y;
+          f2_unpack(sum[i], x, y);
+          l[i] += x + y;
         }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[half]);
       }
       if (ok && nb > 0) {
         ok = mbar_wait_bounded(&o_full[half], 0);
@@ -379,32 +431,46 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tc_fence_after();
       }
       if (ok) {
-        const float inv = m != -INFINITY ? 1.f / l : 0.f;  // no key seen: zeros
-        char* dst = a.out + (first + tok) * a.ld_o +
-                    static_cast<int64_t>(hk * w.group + p - tok * w.group) * (2 * D);
+        char* dst[2];
+        float inv[2];
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int d = 1; d < 4; d <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
+          inv[i] = m[i] != -INFINITY ? 1.f / l[i] : 0.f;  // no key seen: zeros
+          const uint32_t p = p0 + 128 * half + r0 + 8 * i, tok = w.by_group.div(have[i] ? p : 0u);
+          dst[i] = a.out + (first + tok) * a.ld_o +
+                   static_cast<int64_t>(hk * w.group + p - tok * w.group) * (2 * D);
+        }
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
           float o[32];
           if (nb > 0) {
-            tmem_ld_32x32b_x32_nowait(to + 32 * c, o);
+            tmem_ld_16x256b_x8_nowait(to + 64 * c, o);
             tmem_wait_ld(o);
           }
-          if (!have) continue;
 #pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (m != -INFINITY) {
-              v.x = pack2<DT>(o[k] * inv, o[k + 1] * inv);
-              v.y = pack2<DT>(o[k + 2] * inv, o[k + 3] * inv);
-              v.z = pack2<DT>(o[k + 4] * inv, o[k + 5] * inv);
-              v.w = pack2<DT>(o[k + 6] * inv, o[k + 7] * inv);
+          for (int i = 0; i < 2; ++i) {
+            // the four threads of a row trade their pieces of four repetitions,
+            // so that each stores 16 bytes: thread t4 those of repetition 4 q + t4
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t v[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float* e = o + 4 * (4 * q + k) + 2 * i;
+                v[k] = m[i] != -INFINITY ? pack2<DT>(e[0] * inv[i], e[1] * inv[i]) : 0u;
+              }
+              quad_transpose(v, t4);
+              if (have[i])
+                *reinterpret_cast<uint4*>(dst[i] + 128 * c + 64 * q + 16 * t4) =
+                    make_uint4(v[0], v[1], v[2], v[3]);
             }
-            *reinterpret_cast<uint4*>(dst + 64 * c + 2 * k) = v;
           }
         }
       }
     }
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // ------------------------------------------------------- MMA issuer
     if (lane == 0 && nb > 0) {
       const uint32_t id_s = tw_idesc(DT == kBF16, kTileKeys);
@@ -419,10 +485,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         umma_commit(&s_full[h]);
       };
-      auto pv = [&](int h, int slot, int part, bool add) {
+      auto pv = [&](int h, int slot, bool add) {
         const uint32_t va = sm + L::kOffKV + slot * L::kHalf;
 #pragma unroll
-        for (int x = 4 * part; x < 4 * part + 4; ++x)
+        for (int x = 0; x < kTileKeys / 16; ++x)
           umma_f16_tmem_a(tmem + 256 + 128 * h, tmem + 128 * h + 8 * x,
                           umma_desc_sw128(va + 2048 * x, L::kBlk, 1024), id_o, add || x > 0);
       };
@@ -453,14 +519,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           next();
         }
         for (int h = 0; h < halves && ok; ++h) {
-          ok = mbar_wait_bounded(&p_full[2 * h], j & 1);
+          ok = mbar_wait_bounded(&p_full[h], j & 1);
           if (!ok) break;
           tc_fence_after();
-          pv(h, sv, 0, j > 0);
-          ok = mbar_wait_bounded(&p_full[2 * h + 1], j & 1);
-          if (!ok) break;
-          tc_fence_after();
-          pv(h, sv, 1, true);
+          pv(h, sv, j > 0);
           if (h + 1 == halves) umma_commit(&empty[sv]);
           if (more) {
             qk(h, sk);
@@ -476,7 +538,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     // ------------------------------------------------- K / V producer
     const uint32_t boxes = kTileKeys / a.box;
     const uint32_t box_bytes = a.box * 128;  // of one 64-element column block
@@ -546,7 +608,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
