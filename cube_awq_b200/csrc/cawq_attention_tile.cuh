@@ -14,21 +14,26 @@
 //             (with a row a thread and four warps a half a block took 2400
 //             cycles, most of them latency; the tensor cores need 1024)
 //   16        tensor memory, one thread issues every MMA
-//   17        the producer: K_j and V_j of block j through one ring of
-//             128-key stages (TMA, 128-byte swizzle; one box per page, or per
-//             power of two that divides the page)
-// Tensor memory: S_0, S_1 (128 fp32 columns each), O_0, O_1 (D each). The
-// issuing thread's order is S_0(0) S_1(0), then per block PV_0(j) S_0(j + 1)
-// PV_1(j) S_1(j + 1): while the softmax of one half works, the tensor cores do
-// the other half's products. The weights P, rounded to the operand type, go
-// back into tensor memory over the S they came from and are the A operand of
-// PV; V, which lies key by key, is its MN-major B operand.
+//   17-19     the producers: K_j and V_j of block j through one ring of
+//             128-key stages (TMA, 128-byte swizzle; a box is 64 elements of
+//             one page's keys, or of a power of two of them that divides the
+//             page). Pages of 16 make 16 boxes a stage, which one warp issues
+//             in about 1700 cycles: the loads alone took 407 of 544 us then.
+// Tensor memory: one slot for the scores S of a block and half (128 fp32
+// columns), the weights P_0, P_1 (64 columns, the operand type), O_0, O_1 (D
+// fp32 columns each). P is the A operand of the second product from there; V,
+// which lies key by key, its MN-major B operand. The softmax warps move S to
+// registers at once and free the slot, so that the halves take turns with it:
+// the issuing thread's order is S_0(0) S_1(0), then per block S_0(j + 1)
+// PV_0(j) S_1(j + 1) PV_1(j), and a half's softmax of one block runs while the
+// tensor cores do three products, its own next scores among them. (With S_h
+// and P_h in one place, S_h(j + 1) had to wait for PV_h(j) and a block took
+// softmax + two products, 3900 cycles; 8192 tokens 544 us.)
 //
 // The running maximum m moves only when a row's block maximum exceeds it by
 // more than 2^8: p stays below 2^8 either way, nothing overflows (the sums are
 // fp32, f16 holds 65504), and the row's O is rescaled a few times per row
-// instead of once per block. MMAs complete in order, so when S(j) is there,
-// PV(j - 1) has been added to O and the softmax warps may rescale it.
+// instead of once per block. It does so once PV(j - 1) has been added.
 //
 // Stale memory. Pages that no row of the tile needs (past the end, before the
 // window) are not read: their boxes are requested outside the tensor and
@@ -49,7 +54,8 @@ namespace cawq {
 
 constexpr int kTileRows = 256;
 constexpr int kTileKeys = 128;
-constexpr int kTileThreads = 576;
+constexpr int kTileThreads = 640;
+constexpr int kTileLoaders = 3;  // warps that issue the loads of a stage
 constexpr float kTileSlack = 8.f;  // log2 of how far a row's maximum may be exceeded
 constexpr int kTilePoly = 3;       // of 8 pairs of weights, how many take exp2_poly
 
@@ -167,10 +173,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBars);
   uint64_t* empty = full + NS;
   uint64_t* q_full = empty + NS;
-  uint64_t* s_full = q_full + 1;  // [2]
-  uint64_t* p_full = s_full + 2;  // [2]
-  uint64_t* o_full = p_full + 2;  // [2]
-  uint64_t* drain = o_full + 2;
+  uint64_t* s_full = q_full + 1;   // [2]: the slot holds the scores of half h
+  uint64_t* s_free = s_full + 2;   // they are in registers
+  uint64_t* p_full = s_free + 1;   // [2]: the weights are written, O is rescaled
+  uint64_t* pv_done = p_full + 2;  // [2]: PV_h(j) is complete
+  uint64_t* drain = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   __shared__ uint32_t s_bad[8], s_sum[kTileThreads / 32], s_seq, s_tile;
   const AttWork& w = a.w;
@@ -238,15 +245,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], kTileLoaders);
       mbar_init(&empty[s], 1);
     }
     mbar_init(q_full, 512);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 256);
-      mbar_init(&o_full[i], 1);
+      mbar_init(&pv_done[i], 1);
     }
+    mbar_init(s_free, 256);
     mbar_init(drain, 1);
     fence_mbarrier_init();
     fence_proxy_async_smem();
@@ -290,7 +298,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // this thread's rows r0 and r0 + 8 of the half, columns 8 j + 2 (lane % 4), + 1
       const int t4 = lane & 3, r0 = 32 * (warp & 3) + 16 * ((warp >> 2) & 1) + (lane >> 2);
       const uint32_t lanes = static_cast<uint32_t>(r0 & ~15) << 16;
-      const uint32_t ts = tmem + lanes + 128 * half;  // scores; the weights over their first half
+      const uint32_t ts = tmem + lanes, tp = tmem + lanes + 128 + 64 * half;
       const uint32_t to = tmem + lanes + 256 + 128 * half;
       const float sl = a.scale_log2, slack = kTileSlack / sl;
       const uint64_t sl2 = f2_pack(sl, sl);
@@ -325,6 +333,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const bool cut = !__all_sync(0xffffffffu, open);
         tmem_wait_ld(s[0]);
         tmem_wait_ld(s[1]);
+        tc_fence_before();
+        mbar_arrive(s_free);
         if (cut) {
           // a row's visible keys as bits: up to its position, and in the window
           // or among the sinks
@@ -379,6 +389,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             m[i] = mn;
           }
           if (j > 0) {
+            ok = mbar_wait_bounded(&pv_done[half], (j - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               float o[8];
@@ -413,8 +427,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             sum[k & 1] = f2_add(sum[k & 1], f2_pack(x, y));
             pk[k] = pack2<DT>(x, y);
           }
-          tmem_st_16x128b_x8_nowait(ts + 32 * c, pk);
+          if (c == 0 && j > 0) {  // PV(j - 1) has read the weights' place
+            ok = mbar_wait_bounded(&pv_done[half], (j - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          tmem_st_16x128b_x8_nowait(tp + 32 * c, pk);
         }
+        if (!ok) break;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float x, y;
@@ -426,7 +447,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         mbar_arrive(&p_full[half]);
       }
       if (ok && nb > 0) {
-        ok = mbar_wait_bounded(&o_full[half], 0);
+        ok = mbar_wait_bounded(&pv_done[half], (nb - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
@@ -472,134 +493,184 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   } else if (warp == 16) {
     // ------------------------------------------------------- MMA issuer
-    if (lane == 0 && nb > 0) {
+    // the whole warp runs the loop, one thread issues
+    if (nb > 0) {
+      const bool leader = elect_one();
       const uint32_t id_s = tw_idesc(DT == kBF16, kTileKeys);
       constexpr uint32_t id_o = umma_idesc_f16(DT == kBF16, 128, D);
       auto qk = [&](int h, int slot) {
-        const uint32_t qa = sm + h * L::kHalf, ka = sm + L::kOffKV + slot * L::kHalf;
+        const uint64_t qd = umma_desc_sw128(sm + h * L::kHalf, 16, 1024);
+        const uint64_t kd = umma_desc_sw128(sm + L::kOffKV + slot * L::kHalf, 16, 1024);
+        if (leader) {
 #pragma unroll
-        for (int x = 0; x < D / 16; ++x) {
-          const uint32_t o = (x >> 2) * L::kBlk + 32 * (x & 3);
-          umma_f16(tmem + 128 * h, umma_desc_sw128(qa + o, 16, 1024),
-                   umma_desc_sw128(ka + o, 16, 1024), id_s, x > 0);
+          for (int x = 0; x < D / 16; ++x) {  // descriptors count 16-byte units
+            const uint64_t o = ((x >> 2) * L::kBlk + 32 * (x & 3)) >> 4;
+            umma_f16(tmem, qd + o, kd + o, id_s, x > 0);
+          }
+          umma_commit(&s_full[h]);
         }
-        umma_commit(&s_full[h]);
+        __syncwarp();
       };
       auto pv = [&](int h, int slot, bool add) {
-        const uint32_t va = sm + L::kOffKV + slot * L::kHalf;
+        const uint64_t vd = umma_desc_sw128(sm + L::kOffKV + slot * L::kHalf, L::kBlk, 1024);
+        if (leader) {
 #pragma unroll
-        for (int x = 0; x < kTileKeys / 16; ++x)
-          umma_f16_tmem_a(tmem + 256 + 128 * h, tmem + 128 * h + 8 * x,
-                          umma_desc_sw128(va + 2048 * x, L::kBlk, 1024), id_o, add || x > 0);
+          for (int x = 0; x < kTileKeys / 16; ++x)
+            umma_f16_tmem_a(tmem + 256 + 128 * h, tmem + 128 + 64 * h + 8 * x, vd + 128 * x, id_o,
+                            add || x > 0);
+          umma_commit(&pv_done[h]);
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (leader) umma_commit(bar);
+        __syncwarp();
+      };
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity)) != 0;
       };
       const int halves = two ? 2 : 1;
+      // stages in the producer's order: K_0, then K_{j+1}, V_j
       int slot = 0;
       uint32_t par = 0;
-      auto next = [&]() {
+      auto stage = [&](int& s) {  // the next stage, once it is loaded
+        s = slot;
+        const bool ok = wait(&full[slot], par);
         if (++slot == NS) {
           slot = 0;
           par ^= 1u;
         }
+        return ok;
       };
-      bool ok = mbar_wait_bounded(q_full, 0) && mbar_wait_bounded(&full[0], 0);
-      if (ok) {
+      uint32_t scores = 0;  // score products issued; each needs the slot of the one before
+      auto slot_free = [&]() { return scores == 0 || wait(s_free, (scores - 1) & 1); };
+      int sk = 0, sv = 0;
+      bool ok = wait(q_full, 0) && stage(sk);
+      for (int h = 0; h < halves && ok; ++h) {
+        ok = slot_free();
+        if (!ok) break;
         tc_fence_after();
-        for (int h = 0; h < halves; ++h) qk(h, 0);
-        umma_commit(&empty[0]);
-        next();
+        qk(h, sk);
+        ++scores;
       }
+      if (ok) commit(&empty[sk]);
       for (int j = 0; j < nb && ok; ++j) {
-        const int sv = slot;
-        ok = mbar_wait_bounded(&full[sv], par);
-        next();
-        const int sk = slot;
         const bool more = j + 1 < nb;
-        if (more) {
-          ok = ok && mbar_wait_bounded(&full[sk], par);
-          next();
-        }
+        if (more) ok = stage(sk);
         for (int h = 0; h < halves && ok; ++h) {
-          ok = mbar_wait_bounded(&p_full[h], j & 1);
+          if (more) {
+            ok = slot_free();
+            if (!ok) break;
+            tc_fence_after();
+            qk(h, sk);
+            ++scores;
+            if (h + 1 == halves) commit(&empty[sk]);
+          }
+          if (h == 0) ok = stage(sv);
+          ok = ok && wait(&p_full[h], j & 1);
           if (!ok) break;
           tc_fence_after();
           pv(h, sv, j > 0);
-          if (h + 1 == halves) umma_commit(&empty[sv]);
-          if (more) {
-            qk(h, sk);
-            if (h + 1 == halves) umma_commit(&empty[sk]);
-          } else {
-            umma_commit(&o_full[h]);
-          }
+          if (h + 1 == halves) commit(&empty[sv]);
         }
       }
       if (!ok) {
-        umma_commit(drain);
+        commit(drain);
         mbar_wait_bounded(drain, 0);
       }
     }
     __syncwarp();
-  } else if (warp == 17) {
-    // ------------------------------------------------- K / V producer
-    const uint32_t boxes = kTileKeys / a.box;
-    const uint32_t box_bytes = a.box * 128;  // of one 64-element column block
+  } else {
+    // ------------------------------------------------ K / V producers
+    const int loader = warp - 17;
+    const uint32_t boxes = kTileKeys / a.box;  // of a block; each has D / 64 column blocks
+    const uint32_t box_bytes = a.box * 128;
     const int seen = min(len, pos_hi + 1);
     int issued = 0;
     bool ok = true;
-    for (int j = 0; j < nb && ok; ++j) {
-      const int key = block_key(j) + static_cast<int>(lane * a.box);  // this lane's box
-      const bool need = lane < boxes && key < seen &&
-                        (key + static_cast<int>(a.box) > start || key < min(w.sinks, start));
-      int page = -1, in_page = 0;
-      if (need) {
-        const uint32_t pg = w.kv.page.div(key);
-        page = w.kv.table[b * w.kv.ld_table + pg];
-        in_page = key - static_cast<int>(pg * w.kv.page.d);
-      }
-      const bool there = static_cast<uint32_t>(page) < w.kv.pages;
+    // lane i < boxes looks up box i of a block: its page (one block ahead of
+    // its use), and where the sequence ends
+    auto needed = [&](int j) {
+      const int key = block_key(j) + static_cast<int>(lane * a.box);
+      return lane < boxes && key < seen &&
+             (key + static_cast<int>(a.box) > start || key < min(w.sinks, start));
+    };
+    auto fetch = [&](int j) -> int {
+      if (j >= nb || !needed(j)) return -1;
+      return w.kv.table[b * w.kv.ld_table + w.kv.page.div(block_key(j) + lane * a.box)];
+    };
+    struct Box {
+      int key, page, in_page;
+      uint32_t bad, cuts;
+    };
+    auto find = [&](int j, int page) {
+      Box x;
+      x.key = block_key(j) + static_cast<int>(lane * a.box);
+      const bool need = needed(j), there = static_cast<uint32_t>(page) < w.kv.pages;
       const uint32_t gone = __ballot_sync(0xffffffffu, need && !there);
       if (gone != 0 && lane == 0) atomicOr(&g_cawq_device_error, kErrCache);
       // the same by groups of 8 keys
-      const uint32_t bad = __ballot_sync(0xffffffffu, lane < 16 && (gone >> (8 * lane / a.box) & 1));
-      const bool cut = there && key + static_cast<int>(a.box) > len;  // ends inside the box
-      const uint32_t cuts = __ballot_sync(0xffffffffu, cut);
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const int slot = issued % NS, use = issued / NS;
-        if (use > 0) ok = mbar_wait_bounded(&empty[slot], (use - 1) & 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint32_t dst = L::kOffKV + slot * L::kHalf;
-        uint32_t bytes = L::kHalf;
-        if (kv == 1 && cuts != 0) {
-          // the values of the last page, with zeros past the sequence's end
-          const int from = __ffs(cuts) - 1;
-          const int pg = __shfl_sync(0xffffffffu, page, from);
-          const int ip = __shfl_sync(0xffffffffu, in_page, from);
-          const int left = len - __shfl_sync(0xffffffffu, key, from);
-          const char* src = w.kv.v + pg * w.kv.sp + hk * w.kv.sh + ip * w.kv.st;
-          for (uint32_t i = lane; i < a.box * (D / 8); i += 32) {
-            const uint32_t r = i / (D / 8), c = i % (D / 8), rr = from * a.box + r;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (static_cast<int>(r) < left)
-              v = *reinterpret_cast<const uint4*>(src + r * w.kv.st + 16 * c);
-            *reinterpret_cast<uint4*>(smem + dst + (c >> 3) * L::kBlk + rr * 128 +
-                                      (((c & 7) ^ (rr & 7)) << 4)) = v;
-          }
-          fence_proxy_async_smem();
-          bytes -= CB * box_bytes;
+      x.bad = __ballot_sync(0xffffffffu, lane < 16 && (gone >> (8 * lane / a.box) & 1));
+      x.cuts = __ballot_sync(0xffffffffu,
+                             need && there && x.key + static_cast<int>(a.box) > len);
+      // past the last page: the box is outside the tensor and arrives as zeros
+      x.page = there ? page : static_cast<int>(w.kv.pages);
+      x.in_page = need ? x.key - static_cast<int>(w.kv.page.div(x.key) * w.kv.page.d) : 0;
+      return x;
+    };
+    auto load = [&](const Box& x, bool values) {
+      const int slot = issued % NS, use = issued / NS;
+      if (use > 0) ok = mbar_wait_bounded(&empty[slot], (use - 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      const uint32_t dst = L::kOffKV + slot * L::kHalf;
+      // this lane's box and column block: lane of all loaders' lanes
+      const uint32_t item = lane * kTileLoaders + loader, box = item / CB, h = item % CB;
+      const int page = __shfl_sync(0xffffffffu, x.page, box & 31);
+      const int in_page = __shfl_sync(0xffffffffu, x.in_page, box & 31);
+      const uint32_t cuts = values ? x.cuts : 0u;
+      const bool mine = box < boxes && !(cuts >> box & 1);
+      const uint32_t count = __popc(__ballot_sync(0xffffffffu, mine));
+      if (cuts != 0 && loader == 0) {
+        // the values of the last page, with zeros past the sequence's end
+        const int from = __ffs(cuts) - 1;
+        const int pg = __shfl_sync(0xffffffffu, x.page, from);
+        const int ip = __shfl_sync(0xffffffffu, x.in_page, from);
+        const int left = len - __shfl_sync(0xffffffffu, x.key, from);
+        const char* src = w.kv.v + pg * w.kv.sp + hk * w.kv.sh + ip * w.kv.st;
+        for (uint32_t i = lane; i < a.box * (D / 8); i += 32) {
+          const uint32_t r = i / (D / 8), c = i % (D / 8), rr = from * a.box + r;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (static_cast<int>(r) < left)
+            v = *reinterpret_cast<const uint4*>(src + r * w.kv.st + 16 * c);
+          *reinterpret_cast<uint4*>(smem + dst + (c >> 3) * L::kBlk + rr * 128 +
+                                    (((c & 7) ^ (rr & 7)) << 4)) = v;
         }
-        if (kv == 0 && lane == 0) s_bad[j & 7] = bad;
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&full[slot], bytes);
-        __syncwarp();
-        if (lane < boxes && !(kv == 1 && cut)) {
-#pragma unroll
-          for (int h = 0; h < CB; ++h)
-            tma_load_4d(sm + dst + h * L::kBlk + lane * box_bytes, kv ? &tm_v : &tm_k, 64 * h,
-                        in_page, static_cast<int>(hk),
-                        there ? page : static_cast<int>(w.kv.pages), &full[slot]);
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_expect_tx(&full[slot], count * box_bytes);
+      __syncwarp();
+      if (mine)
+        tma_load_4d(sm + dst + h * L::kBlk + box * box_bytes, values ? &tm_v : &tm_k, 64 * h,
+                    in_page, static_cast<int>(hk), page, &full[slot]);
+      ++issued;
+    };
+    if (nb > 0) {
+      Box now = find(0, fetch(0));
+      int page = fetch(1);
+      if (loader == 0 && lane == 0) s_bad[0] = now.bad;
+      load(now, false);
+      for (int j = 0; j < nb && ok; ++j) {
+        Box next = now;
+        if (j + 1 < nb) {
+          next = find(j + 1, page);
+          page = fetch(j + 2);
+          if (loader == 0 && lane == 0) s_bad[(j + 1) & 7] = next.bad;
+          load(next, false);
         }
-        ++issued;
+        if (ok) load(now, true);
+        now = next;
       }
     }
     if (!ok)  // copies in flight end before the CTA does
