@@ -13,22 +13,21 @@
 //   0-7, 8-15 softmax of half 0 and 1: 16 rows a warp, four threads a row
 //             (with a row a thread and four warps a half a block took 2400
 //             cycles, most of them latency; the tensor cores need 1024)
-//   16        tensor memory, one thread issues every MMA
-//   17-19     the producers: K_j and V_j of block j through one ring of
-//             128-key stages (TMA, 128-byte swizzle; a box is 64 elements of
-//             one page's keys, or of a power of two of them that divides the
-//             page). Pages of 16 make 16 boxes a stage, which one warp issues
-//             in about 1700 cycles: the loads alone took 407 of 544 us then.
+//   16, 17    tensor memory; one thread each issues the score products and the
+//             second products (one for both spent its waits and commits one
+//             after the other while the tensor cores idled)
+//   18, 19    K_j and V_j of block j through one ring of 128-key stages (TMA,
+//             128-byte swizzle; a box is a page's keys, or a power of two of
+//             them that divides the page)
 // Tensor memory: one slot for the scores S of a block and half (128 fp32
 // columns), the weights P_0, P_1 (64 columns, the operand type), O_0, O_1 (D
 // fp32 columns each). P is the A operand of the second product from there; V,
 // which lies key by key, its MN-major B operand. The softmax warps move S to
-// registers at once and free the slot, so that the halves take turns with it:
-// the issuing thread's order is S_0(0) S_1(0), then per block S_0(j + 1)
-// PV_0(j) S_1(j + 1) PV_1(j), and a half's softmax of one block runs while the
-// tensor cores do three products, its own next scores among them. (With S_h
-// and P_h in one place, S_h(j + 1) had to wait for PV_h(j) and a block took
-// softmax + two products, 3900 cycles; 8192 tokens 544 us.)
+// registers at once and free the slot, so that the halves take turns with it
+// and a half's softmax of one block runs while the tensor cores do three
+// products, its own next scores among them. (With S_h and P_h in one place,
+// S_h(j + 1) had to wait for PV_h(j), and a block took the softmax and two
+// products.)
 //
 // The running maximum m moves only when a row's block maximum exceeds it by
 // more than 2^8: p stays below 2^8 either way, nothing overflows (the sums are
@@ -55,14 +54,14 @@ namespace cawq {
 constexpr int kTileRows = 256;
 constexpr int kTileKeys = 128;
 constexpr int kTileThreads = 640;
-constexpr int kTileLoaders = 3;  // warps that issue the loads of a stage
+constexpr int kTileLoaders = 2;  // warps that issue the loads of a stage
 constexpr float kTileSlack = 8.f;  // log2 of how far a row's maximum may be exceeded
-constexpr int kTilePoly = 3;       // of 8 pairs of weights, how many take exp2_poly
 
 template <int D>
 struct TileLayout {
   static constexpr int kHalf = 128 * D * 2;  // 128 rows of q, or keys, or values
-  static constexpr int kBlk = 128 * 128;     // their 64-element column block
+  static constexpr int kBlk = 128 * 128;     // of q: a 64-element column block
+  static constexpr int kGroup = 8 * D * 2;   // of keys, values: 8 of them, by column blocks
   static constexpr int kStages = D == 128 ? 5 : 10;
   static constexpr int kOffKV = 2 * kHalf;
   static constexpr int kOffBars = kOffKV + kStages * kHalf;
@@ -94,42 +93,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// 2^x of two values on the FMA pipe (the special-function unit alone takes as
-// long as the tensor cores here): Cody-Waite reduction x = n + f, |f| <= 1/2,
-// by adding and subtracting 1.5 * 2^23; 2^f by a polynomial that is minimax in
-// relative error on [-1/2, 1/2] (Remez exchange; 7.5e-5 of degree 3, enough
-// for weights that are rounded to bf16's 2^-9, 2.6e-6 of degree 4 for f16);
-// 2^n by adding n to the exponent. x <= 9; below -126 the result is no more
-// than 2^-126 (so also for -inf, where the other pairs get 0).
-template <int DT>
-__device__ __forceinline__ void exp2_poly(uint64_t x2, float& a, float& b) {
-  constexpr float kMagic = 12582912.f;
-  float x, y;
-  f2_unpack(x2, x, y);
-  x = fmaxf(x, -126.f);
-  y = fmaxf(y, -126.f);
-  x2 = f2_pack(x, y);
-  const uint64_t t = f2_add(x2, f2_pack(kMagic, kMagic));
-  const uint64_t n = f2_add(t, f2_pack(-kMagic, -kMagic));
-  const uint64_t f = f2_fma(n, f2_pack(-1.f, -1.f), x2);
-  uint64_t p;
-  if constexpr (DT == kBF16) {
-    p = f2_fma(f2_pack(0.05517167f, 0.05517167f), f, f2_pack(0.24261113f, 0.24261113f));
-    p = f2_fma(p, f, f2_pack(0.69326097f, 0.69326097f));
-    p = f2_fma(p, f, f2_pack(0.99992806f, 0.99992806f));
-  } else {
-    p = f2_fma(f2_pack(0.0095701022f, 0.0095701022f), f, f2_pack(0.055917859f, 0.055917859f));
-    p = f2_fma(p, f, f2_pack(0.24024744f, 0.24024744f));
-    p = f2_fma(p, f, f2_pack(0.69312179f, 0.69312179f));
-    p = f2_fma(p, f, f2_pack(0.99999928f, 0.99999928f));
-  }
-  float pa, pb, ta, tb;
-  f2_unpack(p, pa, pb);
-  f2_unpack(t, ta, tb);
-  a = __uint_as_float(__float_as_uint(pa) + (__float_as_uint(ta) << 23));
-  b = __uint_as_float(__float_as_uint(pb) + (__float_as_uint(tb) << 23));
-}
-
 // 4 x 4 transpose among four neighbouring lanes: v[k] of lane t -> v[t] of lane k.
 __device__ __forceinline__ void quad_transpose(uint32_t (&v)[4], int t) {
 #pragma unroll
@@ -155,10 +118,27 @@ struct TileArgs {
   AttWork w;
   int64_t ld_q, ld_o;
   float scale_log2;   // > 0
-  uint32_t flip;      // 0x80008000 with a negative scale: q's signs turn
+  uint32_t negate;    // the score product's "negate A" bit with a negative scale
   uint32_t least;     // sequences with fewer rows belong to the split kernel
   uint32_t box;       // keys of a TMA box: divides page size and 128, a multiple of 8
+  int64_t heads_per_page;  // page stride / head stride
 };
+
+// Stages of a tile in the producers' order: K_0, then K_{j+1}, V_j.
+__device__ __forceinline__ uint32_t tile_stage_k(int j) { return j == 0 ? 0 : 2 * j - 1; }
+__device__ __forceinline__ uint32_t tile_stage_v(int j, int nb) {
+  return j + 1 < nb ? 2 * j + 2 : 2 * nb - 1;
+}
+
+// Pages as heads: how many head strides a page stride is; 0 where the two do
+// not make one dimension (the split kernel then takes the call).
+inline uint64_t tile_heads_per_page(const PagedView& kv) {
+  if (kv.pages == 0) return 0;
+  if (kv.n_kv == 1 || kv.pages == 1) return kv.n_kv;
+  if (kv.sh <= 0 || kv.sp % kv.sh != 0 || kv.sp / kv.sh < static_cast<int64_t>(kv.n_kv)) return 0;
+  const uint64_t per = static_cast<uint64_t>(kv.sp / kv.sh);
+  return per * (kv.pages + 1) < (1ull << 31) ? per : 0;
+}
 
 template <int DT, int D>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -166,7 +146,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                           const __grid_constant__ CUtensorMap tm_v,
                           const __grid_constant__ TileArgs a) {
   using L = TileLayout<D>;
-  constexpr int NS = L::kStages, CB = D / 64;
+  constexpr int NS = L::kStages;
   constexpr uint32_t kTmemCols = 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -177,8 +157,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* s_free = s_full + 2;   // they are in registers
   uint64_t* p_full = s_free + 1;   // [2]: the weights are written, O is rescaled
   uint64_t* pv_done = p_full + 2;  // [2]: PV_h(j) is complete
-  uint64_t* drain = pv_done + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* drain = pv_done + 2;  // [2]: of the issuers
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   __shared__ uint32_t s_bad[8], s_sum[kTileThreads / 32], s_seq, s_tile;
   const AttWork& w = a.w;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -251,11 +231,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     mbar_init(q_full, 512);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 256);
+      mbar_init(&p_full[i], 8);
       mbar_init(&pv_done[i], 1);
     }
-    mbar_init(s_free, 256);
-    mbar_init(drain, 1);
+    mbar_init(s_free, 8);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     fence_mbarrier_init();
     fence_proxy_async_smem();
     tma_prefetch_desc(&tm_k);
@@ -283,10 +264,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         v = *reinterpret_cast<const uint4*>(
             a.q + (first + tok) * a.ld_q +
             static_cast<int64_t>(hk * w.group + p - tok * w.group) * (2 * D) + 16 * c);
-        v.x ^= a.flip;
-        v.y ^= a.flip;
-        v.z ^= a.flip;
-        v.w ^= a.flip;
       }
       *reinterpret_cast<uint4*>(smem + (r >> 7) * L::kHalf + (c >> 3) * L::kBlk + (r & 127) * 128 +
                                 (((c & 7) ^ (r & 7)) << 4)) = v;
@@ -315,7 +292,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       bool ok = true;
       for (int j = 0; j < nb; ++j) {
-        ok = mbar_wait_bounded(&s_full[half], j & 1);
+        ok = mbar_wait_prompt(&s_full[half], j & 1);
         ok = __all_sync(0xffffffffu, ok);  // tcgen05.ld / st are warp-collective
         if (!ok) break;
         tc_fence_after();
@@ -334,7 +311,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tmem_wait_ld(s[0]);
         tmem_wait_ld(s[1]);
         tc_fence_before();
-        mbar_arrive(s_free);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free);
         if (cut) {
           // a row's visible keys as bits: up to its position, and in the window
           // or among the sinks
@@ -389,7 +367,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             m[i] = mn;
           }
           if (j > 0) {
-            ok = mbar_wait_bounded(&pv_done[half], (j - 1) & 1);
+            ok = mbar_wait_prompt(&pv_done[half], (j - 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
@@ -417,18 +395,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const uint64_t x2 =
                 f2_fma(f2_pack(s[c][2 * k], s[c][2 * k + 1]), sl2, nb2[k & 1]);
             float x, y;
-            if (k * kTilePoly % 8 < kTilePoly) {
-              exp2_poly<DT>(x2, x, y);
-            } else {
-              f2_unpack(x2, x, y);
-              x = exp2_approx(x);
-              y = exp2_approx(y);
-            }
+            f2_unpack(x2, x, y);
+            x = exp2_approx(x);
+            y = exp2_approx(y);
             sum[k & 1] = f2_add(sum[k & 1], f2_pack(x, y));
             pk[k] = pack2<DT>(x, y);
           }
           if (c == 0 && j > 0) {  // PV(j - 1) has read the weights' place
-            ok = mbar_wait_bounded(&pv_done[half], (j - 1) & 1);
+            ok = mbar_wait_prompt(&pv_done[half], (j - 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
@@ -444,10 +418,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_full[half]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[half]);
       }
       if (ok && nb > 0) {
-        ok = mbar_wait_bounded(&pv_done[half], (nb - 1) & 1);
+        ok = mbar_wait_prompt(&pv_done[half], (nb - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
@@ -492,145 +467,126 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
     }
   } else if (warp == 16) {
-    // ------------------------------------------------------- MMA issuer
-    // the whole warp runs the loop, one thread issues
-    if (nb > 0) {
-      const bool leader = elect_one();
-      const uint32_t id_s = tw_idesc(DT == kBF16, kTileKeys);
-      constexpr uint32_t id_o = umma_idesc_f16(DT == kBF16, 128, D);
-      auto qk = [&](int h, int slot) {
-        const uint64_t qd = umma_desc_sw128(sm + h * L::kHalf, 16, 1024);
-        const uint64_t kd = umma_desc_sw128(sm + L::kOffKV + slot * L::kHalf, 16, 1024);
-        if (leader) {
-#pragma unroll
-          for (int x = 0; x < D / 16; ++x) {  // descriptors count 16-byte units
-            const uint64_t o = ((x >> 2) * L::kBlk + 32 * (x & 3)) >> 4;
-            umma_f16(tmem, qd + o, kd + o, id_s, x > 0);
-          }
-          umma_commit(&s_full[h]);
-        }
-        __syncwarp();
-      };
-      auto pv = [&](int h, int slot, bool add) {
-        const uint64_t vd = umma_desc_sw128(sm + L::kOffKV + slot * L::kHalf, L::kBlk, 1024);
-        if (leader) {
-#pragma unroll
-          for (int x = 0; x < kTileKeys / 16; ++x)
-            umma_f16_tmem_a(tmem + 256 + 128 * h, tmem + 128 + 64 * h + 8 * x, vd + 128 * x, id_o,
-                            add || x > 0);
-          umma_commit(&pv_done[h]);
-        }
-        __syncwarp();
-      };
-      auto commit = [&](uint64_t* bar) {
-        if (leader) umma_commit(bar);
-        __syncwarp();
-      };
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity)) != 0;
-      };
-      const int halves = two ? 2 : 1;
-      // stages in the producer's order: K_0, then K_{j+1}, V_j
-      int slot = 0;
-      uint32_t par = 0;
-      auto stage = [&](int& s) {  // the next stage, once it is loaded
-        s = slot;
-        const bool ok = wait(&full[slot], par);
-        if (++slot == NS) {
-          slot = 0;
-          par ^= 1u;
-        }
-        return ok;
-      };
-      uint32_t scores = 0;  // score products issued; each needs the slot of the one before
-      auto slot_free = [&]() { return scores == 0 || wait(s_free, (scores - 1) & 1); };
-      int sk = 0, sv = 0;
-      bool ok = wait(q_full, 0) && stage(sk);
-      for (int h = 0; h < halves && ok; ++h) {
-        ok = slot_free();
+    // ------------------------------------------ issuer of the score products
+    // (the whole warp runs the loop, one thread issues)
+    const bool leader = elect_one();
+    const uint32_t id_s = tw_idesc(DT == kBF16, kTileKeys) | a.negate;
+    const uint64_t qd = umma_desc_sw128(sm, 16, 1024);
+    const uint64_t kd = umma_desc_sw128(sm + L::kOffKV, 16, L::kGroup);
+    const int halves = two ? 2 : 1;
+    uint32_t scores = 0;  // score products issued; each needs the slot of the one before
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && mbar_wait_prompt(bar, parity);
+      ok = __all_sync(0xffffffffu, ok);
+    };
+    if (nb > 0) wait(q_full, 0);
+    for (int j = 0; j < nb && ok; ++j) {
+      const uint32_t st = tile_stage_k(j), slot = st % NS;
+      wait(&full[slot], st / NS & 1);
+      for (int h = 0; h < halves; ++h) {
+        if (scores > 0) wait(s_free, (scores - 1) & 1);
         if (!ok) break;
-        tc_fence_after();
-        qk(h, sk);
         ++scores;
-      }
-      if (ok) commit(&empty[sk]);
-      for (int j = 0; j < nb && ok; ++j) {
-        const bool more = j + 1 < nb;
-        if (more) ok = stage(sk);
-        for (int h = 0; h < halves && ok; ++h) {
-          if (more) {
-            ok = slot_free();
-            if (!ok) break;
-            tc_fence_after();
-            qk(h, sk);
-            ++scores;
-            if (h + 1 == halves) commit(&empty[sk]);
-          }
-          if (h == 0) ok = stage(sv);
-          ok = ok && wait(&p_full[h], j & 1);
-          if (!ok) break;
-          tc_fence_after();
-          pv(h, sv, j > 0);
-          if (h + 1 == halves) commit(&empty[sv]);
+        tc_fence_after();
+        if (leader) {
+          const uint64_t q = qd + h * (L::kHalf >> 4), k = kd + slot * (L::kHalf >> 4);
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x)  // descriptors count 16-byte units
+            umma_f16(tmem, q + 2 * (x & 3) + (x >> 2) * (L::kBlk >> 4),
+                     k + 2 * (x & 3) + (x >> 2) * (1024 >> 4), id_s, x > 0);
+          umma_commit(&s_full[h]);
+          if (h + 1 == halves) umma_commit(&empty[slot]);
         }
-      }
-      if (!ok) {
-        commit(drain);
-        mbar_wait_bounded(drain, 0);
+        __syncwarp();
       }
     }
-    __syncwarp();
-  } else {
-    // ------------------------------------------------ K / V producers
-    const int loader = warp - 17;
-    const uint32_t boxes = kTileKeys / a.box;  // of a block; each has D / 64 column blocks
-    const uint32_t box_bytes = a.box * 128;
-    const int seen = min(len, pos_hi + 1);
-    int issued = 0;
+    if (!ok) {
+      if (leader) umma_commit(&drain[0]);
+      __syncwarp();
+      mbar_wait_bounded(&drain[0], 0);
+    }
+  } else if (warp == 17) {
+    // ----------------------------------------- issuer of the second products
+    const bool leader = elect_one();
+    constexpr uint32_t id_o = umma_idesc_f16(DT == kBF16, 128, D);
+    const uint64_t vd = umma_desc_sw128(sm + L::kOffKV, 1024, L::kGroup);
+    const int halves = two ? 2 : 1;
     bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && mbar_wait_prompt(bar, parity);
+      ok = __all_sync(0xffffffffu, ok);
+    };
+    for (int j = 0; j < nb && ok; ++j) {
+      const uint32_t st = tile_stage_v(j, nb), slot = st % NS;
+      wait(&full[slot], st / NS & 1);
+      for (int h = 0; h < halves; ++h) {
+        wait(&p_full[h], j & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+          const uint32_t o = tmem + 256 + 128 * h, p = tmem + 128 + 64 * h;
+          const uint64_t v = vd + slot * (L::kHalf >> 4);
+#pragma unroll
+          for (int x = 0; x < kTileKeys / 16; ++x)
+            umma_f16_tmem_a(o, p + 8 * x, v + x * (2 * L::kGroup >> 4), id_o, j > 0 || x > 0);
+          umma_commit(&pv_done[h]);
+          if (h + 1 == halves) umma_commit(&empty[slot]);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) {
+      if (leader) umma_commit(&drain[1]);
+      __syncwarp();
+      mbar_wait_bounded(&drain[1], 0);
+    }
+  } else {
+    // ------------------------------------------------- K / V producers
+    const int loader = warp - 18;
+    const uint32_t box_keys = a.box, boxes = kTileKeys / box_keys;  // of a block
+    const uint32_t box_bytes = box_keys * 2 * D;
+    int slot = 0, issued = 0;
+    uint32_t par = 1;  // parity of the slot's last release (a fresh barrier: done)
+    bool ok = true;
+    const int seen = min(len, pos_hi + 1), sinks = min(w.sinks, start);
+    const int32_t* table = w.kv.table + b * w.kv.ld_table;
     // lane i < boxes looks up box i of a block: its page (one block ahead of
     // its use), and where the sequence ends
-    auto needed = [&](int j) {
-      const int key = block_key(j) + static_cast<int>(lane * a.box);
-      return lane < boxes && key < seen &&
-             (key + static_cast<int>(a.box) > start || key < min(w.sinks, start));
-    };
-    auto fetch = [&](int j) -> int {
-      if (j >= nb || !needed(j)) return -1;
-      return w.kv.table[b * w.kv.ld_table + w.kv.page.div(block_key(j) + lane * a.box)];
-    };
     struct Box {
       int key, page, in_page;
+      bool need;
       uint32_t bad, cuts;
     };
-    auto find = [&](int j, int page) {
+    auto fetch = [&](int j) {
       Box x;
-      x.key = block_key(j) + static_cast<int>(lane * a.box);
-      const bool need = needed(j), there = static_cast<uint32_t>(page) < w.kv.pages;
-      const uint32_t gone = __ballot_sync(0xffffffffu, need && !there);
-      if (gone != 0 && lane == 0) atomicOr(&g_cawq_device_error, kErrCache);
-      // the same by groups of 8 keys
-      x.bad = __ballot_sync(0xffffffffu, lane < 16 && (gone >> (8 * lane / a.box) & 1));
-      x.cuts = __ballot_sync(0xffffffffu,
-                             need && there && x.key + static_cast<int>(a.box) > len);
-      // past the last page: the box is outside the tensor and arrives as zeros
-      x.page = there ? page : static_cast<int>(w.kv.pages);
-      x.in_page = need ? x.key - static_cast<int>(w.kv.page.div(x.key) * w.kv.page.d) : 0;
+      x.key = (j < head ? j : main0 + j - head) * kTileKeys + static_cast<int>(lane * box_keys);
+      x.need = j < nb && lane < boxes && x.key < seen &&
+               (x.key + static_cast<int>(box_keys) > start || x.key < sinks);
+      const uint32_t pg = x.need ? w.kv.page.div(x.key) : 0u;
+      x.in_page = x.need ? x.key - static_cast<int>(pg * w.kv.page.d) : 0;
+      x.page = x.need ? table[pg] : -1;
       return x;
     };
+    auto find = [&](Box& x) {
+      const bool there = static_cast<uint32_t>(x.page) < w.kv.pages;
+      const uint32_t gone = __ballot_sync(0xffffffffu, x.need && !there);
+      x.bad = 0;
+      if (gone != 0) {
+        if (lane == 0) atomicOr(&g_cawq_device_error, kErrCache);
+        // the same by groups of 8 keys
+        x.bad = __ballot_sync(0xffffffffu, lane < 16 && (gone >> (8 * lane / box_keys) & 1));
+      }
+      x.cuts = __ballot_sync(0xffffffffu, there && x.key + static_cast<int>(box_keys) > len);
+      // past the last page: the box is outside the tensor and arrives as zeros
+      if (!there) x.page = static_cast<int>(w.kv.pages);
+    };
     auto load = [&](const Box& x, bool values) {
-      const int slot = issued % NS, use = issued / NS;
-      if (use > 0) ok = mbar_wait_bounded(&empty[slot], (use - 1) & 1);
+      ok = ok && mbar_wait_prompt(&empty[slot], par);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       const uint32_t dst = L::kOffKV + slot * L::kHalf;
-      // this lane's box and column block: lane of all loaders' lanes
-      const uint32_t item = lane * kTileLoaders + loader, box = item / CB, h = item % CB;
-      const int page = __shfl_sync(0xffffffffu, x.page, box & 31);
-      const int in_page = __shfl_sync(0xffffffffu, x.in_page, box & 31);
       const uint32_t cuts = values ? x.cuts : 0u;
-      const bool mine = box < boxes && !(cuts >> box & 1);
-      const uint32_t count = __popc(__ballot_sync(0xffffffffu, mine));
       if (cuts != 0 && loader == 0) {
         // the values of the last page, with zeros past the sequence's end
         const int from = __ffs(cuts) - 1;
@@ -638,34 +594,44 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int ip = __shfl_sync(0xffffffffu, x.in_page, from);
         const int left = len - __shfl_sync(0xffffffffu, x.key, from);
         const char* src = w.kv.v + pg * w.kv.sp + hk * w.kv.sh + ip * w.kv.st;
-        for (uint32_t i = lane; i < a.box * (D / 8); i += 32) {
-          const uint32_t r = i / (D / 8), c = i % (D / 8), rr = from * a.box + r;
+        for (uint32_t i = lane; i < box_keys * (D / 8); i += 32) {
+          const uint32_t r = i / (D / 8), c = i % (D / 8), rr = from * box_keys + r;
           uint4 v = make_uint4(0, 0, 0, 0);
           if (static_cast<int>(r) < left)
             v = *reinterpret_cast<const uint4*>(src + r * w.kv.st + 16 * c);
-          *reinterpret_cast<uint4*>(smem + dst + (c >> 3) * L::kBlk + rr * 128 +
-                                    (((c & 7) ^ (rr & 7)) << 4)) = v;
+          *reinterpret_cast<uint4*>(smem + dst + (rr >> 3) * L::kGroup + (c >> 3) * 1024 +
+                                    (rr & 7) * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
         }
         fence_proxy_async_smem();
       }
-      __syncwarp();
+      // the boxes are dealt out to the loaders' lanes
+      const uint32_t box = lane * kTileLoaders + loader;
+      const int page = __shfl_sync(0xffffffffu, x.page, box & 31);
+      const int in_page = __shfl_sync(0xffffffffu, x.in_page, box & 31);
+      const bool mine = box < boxes && !(cuts >> box & 1);
+      const uint32_t count = __popc(__ballot_sync(0xffffffffu, mine));
       if (lane == 0) mbar_arrive_expect_tx(&full[slot], count * box_bytes);
       __syncwarp();
       if (mine)
-        tma_load_4d(sm + dst + h * L::kBlk + box * box_bytes, values ? &tm_v : &tm_k, 64 * h,
-                    in_page, static_cast<int>(hk), page, &full[slot]);
+        tma_load_5d(sm + dst + box * box_bytes, values ? &tm_v : &tm_k, 0, 0, 0, in_page / 8,
+                    static_cast<int>(page * a.heads_per_page + static_cast<int>(hk)), &full[slot]);
+      __syncwarp();
       ++issued;
+      if (++slot == NS) {
+        slot = 0;
+        par ^= 1u;
+      }
     };
     if (nb > 0) {
-      Box now = find(0, fetch(0));
-      int page = fetch(1);
+      Box now = fetch(0), after = fetch(1);
+      find(now);
       if (loader == 0 && lane == 0) s_bad[0] = now.bad;
       load(now, false);
       for (int j = 0; j < nb && ok; ++j) {
-        Box next = now;
+        Box next = after;
         if (j + 1 < nb) {
-          next = find(j + 1, page);
-          page = fetch(j + 2);
+          after = fetch(j + 2);
+          find(next);
           if (loader == 0 && lane == 0) s_bad[(j + 1) & 7] = next.bad;
           load(next, false);
         }
@@ -673,9 +639,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         now = next;
       }
     }
-    if (!ok)  // copies in flight end before the CTA does
+    if (!ok) {  // copies in flight end before the CTA does
       for (int i = max(0, issued - NS); i < issued; ++i)
         mbar_wait_bounded(&full[i % NS], (i / NS) & 1);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -685,19 +652,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 }
 
-// The cache's keys or values as a 4-D tensor: elements, slots, heads, pages.
+// The cache's keys or values as a 5-D tensor: 64 elements, 8 slots, column
+// blocks, groups of 8 slots, heads (those of a page follow those of the page
+// before). A box then lands group by group, column block by column block: one
+// copy per page brings every column. (TMA takes 60 cycles or more for a box
+// however small: with a box per column block, pages of 16 made the loads the
+// bound, 1400 cycles a stage.) False if the strides do not fit.
 inline bool encode_cache(CUtensorMap* map, int dtype, const void* base, const PagedView& kv,
                          uint32_t d, uint32_t box) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return false;
-  const uint64_t dims[4] = {d, kv.page.d, kv.n_kv, kv.pages};
   // an extent of 1 never uses its stride, which may then be anything
-  const uint64_t strides[3] = {static_cast<uint64_t>(kv.page.d > 1 ? kv.st : 2 * d),
-                               static_cast<uint64_t>(kv.n_kv > 1 ? kv.sh : 2 * d),
-                               static_cast<uint64_t>(kv.pages > 1 ? kv.sp : 2 * d)};
-  const uint32_t bx[4] = {64, box, 1, 1}, es[4] = {1, 1, 1, 1};
+  const uint64_t sh = kv.n_kv > 1 || kv.pages > 1 ? kv.n_kv > 1 ? kv.sh : kv.sp : 2 * d;
+  const uint64_t per = tile_heads_per_page(kv);
+  const uint64_t dims[5] = {64, 8, d / 64, kv.page.d / 8, (kv.pages - 1) * per + kv.n_kv};
+  const uint64_t strides[4] = {static_cast<uint64_t>(kv.st), 128, 8 * static_cast<uint64_t>(kv.st), sh};
+  const uint32_t bx[5] = {64, 8, d / 64, box / 8, 1}, es[5] = {1, 1, 1, 1, 1};
   return fn(map, dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-            4, const_cast<void*>(base), dims, strides, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            5, const_cast<void*>(base), dims, strides, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == 0;
 }
@@ -716,10 +688,11 @@ cudaError_t launch_attention_tile_t(const AttentionProblem& p, const PagedView& 
   a.ld_o = static_cast<int64_t>(p.ld_out) * 2;
   // scores of a scale of 0 are all equal: so they are at 1e-30
   a.scale_log2 = std::max(std::abs(p.scale) * kLog2e, 1e-30f);
-  a.flip = p.scale < 0 ? 0x80008000u : 0u;
+  a.negate = p.scale < 0 ? 1u << 13 : 0u;
   a.least = least;
   a.box = 8;
   while (a.box < kTileKeys && kv.page.d % (2 * a.box) == 0) a.box *= 2;
+  a.heads_per_page = static_cast<int64_t>(tile_heads_per_page(kv));
   CUtensorMap mk, mv;
   if (!encode_cache(&mk, DT, kv.k, kv, D, a.box) || !encode_cache(&mv, DT, kv.v, kv, D, a.box))
     return cudaErrorInvalidValue;

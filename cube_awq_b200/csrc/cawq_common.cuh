@@ -158,6 +158,16 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
+// The same for hand-overs that a loop's pace hangs on: 64 tries before the
+// clock is read for the first time (reading it costs the waiter more than the
+// hand-over).
+__device__ __forceinline__ bool mbar_wait_prompt(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_bounded(bar, parity);
+}
+
 // ----------------------------------------------------------------- TMA
 // 2-D tiled bulk tensor load into this CTA's shared memory, completion on an
 // mbarrier (no multicast). c0 is the inner (contiguous) coordinate.
@@ -170,14 +180,14 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
-// 4-D tiled bulk tensor load, as above. A box outside the tensor's extent is
+// 5-D tiled bulk tensor load, as above. A box outside the tensor's extent is
 // filled with zeros and counts its whole bytes.
-__device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const CUtensorMap* map, int c0,
-                                            int c1, int c2, int c3, uint64_t* bar) {
+__device__ __forceinline__ void tma_load_5d(uint32_t smem_dst, const CUtensorMap* map, int c0,
+                                            int c1, int c2, int c3, int c4, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3),
+      "cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4),
       "r"(smem_u32(bar))
       : "memory");
 }
@@ -197,6 +207,20 @@ __device__ __forceinline__ void bulk_load_1d(void* smem_dst, const void* src, ui
 // barrier `id` (1..15; 0 is __syncthreads).
 __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t count) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
+}
+
+// The same barrier; true for all if the predicate is for one.
+__device__ __forceinline__ bool named_bar_or(uint32_t id, bool v, uint32_t count = 64) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(count), "r"(static_cast<uint32_t>(v))
+      : "memory");
+  return r != 0;
 }
 
 // Address of output element (row, col): columns [0, c1) live in p0 (row

@@ -202,7 +202,7 @@ static cawq_status attention(const void* q, void* out, const cawq_paged_kv* kv, 
                               dev.sm_count, dev.device, static_cast<cudaStream_t>(stream)};
   const PagedView view = paged_view(*kv, 2, decode);
   cudaError_t e;
-  if (decode || kv->pages == 0) {
+  if (decode || tile_heads_per_page(view) == 0) {
     e = launch_attention_split(p, view);
   } else {
     e = launch_attention_tile(p, view, 0);
