@@ -159,69 +159,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* pv_done = p_full + 2;  // [2]: PV_h(j) is complete
   uint64_t* drain = pv_done + 2;  // [2]: of the issuers
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
-  __shared__ uint32_t s_bad[8], s_sum[kTileThreads / 32], s_seq, s_tile;
+  __shared__ uint32_t s_bad[8], s_sum[kTileThreads / 32];
+  __shared__ struct {
+    uint32_t seq, tile;
+    int first, count, len;
+  } s_tile;
   const AttWork& w = a.w;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-  pdl_wait();
-  pdl_launch_dependents();
-  // ---- which tile: the sequences' tiles in order, a sequence's last tile first
-  // (the later a causal tile, the longer it takes)
-  const uint32_t index = blockIdx.x / w.kv.n_kv, hk = blockIdx.x - index * w.kv.n_kv;
-  {
-    auto tiles = [&](uint32_t b) -> uint32_t {
-      int first, count;
-      w.kv.rows(b, w.tokens, &first, &count);
-      const uint32_t rows = static_cast<uint32_t>(count) * w.group;
-      return rows >= a.least ? (rows + kTileRows - 1) / kTileRows : 0u;
-    };
-    const uint32_t per = (w.kv.batch + kTileThreads - 1) / kTileThreads;
-    const uint32_t b0 = min(w.kv.batch, tid * per), b1 = min(w.kv.batch, b0 + per);
-    uint32_t n = 0;
-    for (uint32_t b = b0; b < b1; ++b) n += tiles(b);
-    uint32_t inc = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    if (lane == 31) s_sum[warp] = inc;
-    if (tid == 0) s_seq = 0xffffffffu;
-    __syncthreads();
-    uint32_t at = inc - n;
-    for (int i = 0; i < warp; ++i) at += s_sum[i];
-    if (index >= at && index < at + n) {
-      uint32_t b = b0;
-      for (;; ++b) {
-        const uint32_t t = tiles(b);
-        if (index < at + t) {
-          s_tile = t - 1 - (index - at);
-          break;
-        }
-        at += t;
-      }
-      s_seq = b;
-    }
-    __syncthreads();
-  }
-  const uint32_t b = s_seq;
-  if (b == 0xffffffffu) return;  // the grid is sized for the most tiles there can be
-
-  // ---- the tile's rows and key blocks
-  int first, count;
-  w.kv.rows(b, w.tokens, &first, &count);
-  const int len = w.kv.len(b);
-  const uint32_t rows = static_cast<uint32_t>(count) * w.group;
-  const uint32_t p0 = s_tile * kTileRows;
-  const bool two = p0 + 128 < rows;
-  const int shift = len - count;  // position of the first new token
-  const int pos_lo = shift + static_cast<int>(w.by_group.div(p0));
-  const int pos_hi = shift + static_cast<int>(w.by_group.div(min(p0 + kTileRows, rows) - 1));
-  const int start = w.window > 0 ? max(0, pos_lo - w.window + 1) : 0;
-  const int head = (min(w.sinks, start) + kTileKeys - 1) / kTileKeys;  // blocks that hold sinks
-  const int main0 = max(start / kTileKeys, head);
-  const int nb = pos_hi < 0 ? 0 : head + max(0, pos_hi / kTileKeys - main0 + 1);
-  auto block_key = [&](int j) { return (j < head ? j : main0 + j - head) * kTileKeys; };
 
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
@@ -243,9 +187,64 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tma_prefetch_desc(&tm_v);
   }
   if (warp == 16) tmem_alloc(tmem_slot, kTmemCols);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  pdl_wait();
+  pdl_launch_dependents();
+  // ---- which tile: the sequences' tiles in order, a sequence's last tile first
+  // (the later a causal tile, the longer it takes)
+  const uint32_t index = blockIdx.x / w.kv.n_kv, hk = blockIdx.x - index * w.kv.n_kv;
+  {
+    auto tiles = [&](uint32_t b, int* first, int* count, int* len) -> uint32_t {
+      w.kv.rows(b, w.tokens, first, count);
+      *len = w.kv.len(b);
+      const uint32_t rows = static_cast<uint32_t>(*count) * w.group;
+      return rows >= a.least ? (rows + kTileRows - 1) / kTileRows : 0u;
+    };
+    const uint32_t per = (w.kv.batch + kTileThreads - 1) / kTileThreads;
+    const uint32_t b0 = min(w.kv.batch, tid * per), b1 = min(w.kv.batch, b0 + per);
+    int first = 0, count = 0, len = 0;
+    uint32_t n = 0, last = 0;
+    for (uint32_t b = b0; b < b1; ++b) n += last = tiles(b, &first, &count, &len);
+    uint32_t inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) s_sum[warp] = inc;
+    if (tid == 0) s_tile.seq = 0xffffffffu;
+    tc_fence_before();
+    __syncthreads();
+    uint32_t at = inc - n;
+    for (int i = 0; i < warp; ++i) at += s_sum[i];
+    if (index >= at && index < at + n) {
+      uint32_t b = b1 - 1;  // the usual case: a sequence a thread
+      if (per > 1)
+        for (b = b0; index >= at + (last = tiles(b, &first, &count, &len)); ++b) at += last;
+      s_tile = {b, last - 1 - (index - at), first, count, len};
+    }
+    __syncthreads();
+    tc_fence_after();
+  }
+  const uint32_t b = s_tile.seq;
+  if (b == 0xffffffffu) {  // the grid is sized for the most tiles there can be
+    if (warp == 16) tmem_dealloc(*tmem_slot, kTmemCols);
+    return;
+  }
+
+  // ---- the tile's rows and key blocks
+  const int first = s_tile.first, count = s_tile.count, len = s_tile.len;
+  const uint32_t rows = static_cast<uint32_t>(count) * w.group;
+  const uint32_t p0 = s_tile.tile * kTileRows;
+  const bool two = p0 + 128 < rows;
+  const int shift = len - count;  // position of the first new token
+  const int pos_lo = shift + static_cast<int>(w.by_group.div(p0));
+  const int pos_hi = shift + static_cast<int>(w.by_group.div(min(p0 + kTileRows, rows) - 1));
+  const int start = w.window > 0 ? max(0, pos_lo - w.window + 1) : 0;
+  const int head = (min(w.sinks, start) + kTileKeys - 1) / kTileKeys;  // blocks that hold sinks
+  const int main0 = max(start / kTileKeys, head);
+  const int nb = pos_hi < 0 ? 0 : head + max(0, pos_hi / kTileKeys - main0 + 1);
+  auto block_key = [&](int j) { return (j < head ? j : main0 + j - head) * kTileKeys; };
+
   const uint32_t tmem = *tmem_slot;
   const uint32_t sm = smem_u32(smem);
 
@@ -254,20 +253,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int half = warp >> 3;
     // both halves' rows of q into shared memory, K-major with 128-byte swizzle
     constexpr int CPR = D / 8;
-#pragma unroll 4
-    for (int i = tid; i < kTileRows * CPR; i += 512) {
-      const uint32_t r = i / CPR, c = i % CPR, p = p0 + r;
-      if (r >= 128 && !two) break;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (p < rows) {
-        const uint32_t tok = w.by_group.div(p);
-        v = *reinterpret_cast<const uint4*>(
-            a.q + (first + tok) * a.ld_q +
-            static_cast<int64_t>(hk * w.group + p - tok * w.group) * (2 * D) + 16 * c);
-      }
-      *reinterpret_cast<uint4*>(smem + (r >> 7) * L::kHalf + (c >> 3) * L::kBlk + (r & 127) * 128 +
-                                (((c & 7) ^ (r & 7)) << 4)) = v;
+#pragma unroll 8
+    for (uint32_t r = tid / CPR; r < (two ? 256u : 128u); r += 512 / CPR) {
+      const uint32_t c = tid % CPR, p = p0 + r, tok = w.by_group.div(p);
+      cp_async_16(sm + (r >> 7) * L::kHalf + (c >> 3) * L::kBlk + (r & 127) * 128 +
+                      (((c & 7) ^ (r & 7)) << 4),
+                  p < rows ? a.q + (first + tok) * a.ld_q +
+                                 static_cast<int64_t>(hk * w.group + p - tok * w.group) * (2 * D) +
+                                 16 * c
+                           : a.q,
+                  p < rows ? 16 : 0);
     }
+    cp_async_commit();
+    cp_async_wait<0>();
     fence_proxy_async_smem();
     mbar_arrive(q_full);
 
