@@ -43,6 +43,9 @@ constexpr int kAttStages = 3;
 // long ones left the CTAs with the short ones last (64 sequences of 1 to 8000
 // tokens, 28 / 4 heads: 62 us).
 constexpr uint32_t kAttRowCost = 2;
+// Query rows of a (sequence, kv head) that are few: always up to the first
+// number; up to the second if there are that many keys to a row to split.
+constexpr uint32_t kAttFew = 16, kAttFewLong = 128, kAttFewKeys = 40;
 constexpr int kAttMaxCtas = 320;  // most CTAs of a launch (two per SM)
 
 template <int D>
@@ -101,7 +104,16 @@ struct AttWork {
   uint32_t tokens, group, row_tile;  // group = n_q / n_kv, row_tile = NR
   FastDiv by_group;
   int window, sinks;
-  uint32_t most_rows;  // sequences with more rows belong to the tile kernel
+  bool shared;  // the tile kernel takes the sequences whose rows are not few
+
+  // Few rows are bound by their keys' bytes and gain from the split; many by
+  // the tensor cores. Per call, us split / tiles (D = 128, bf16, one
+  // sequence): 64 rows, 8 kv heads at 500 / 3000 / 20000 keys 22 / 31 / 101
+  // against 11 / 35 / 187; 128 rows 25 / 45 / 181 against 12 / 35 / 188.
+  __device__ __forceinline__ static bool few(uint32_t rows, int len) {
+    return rows <= kAttFew ||
+           (rows <= kAttFewLong && static_cast<uint32_t>(len) >= kAttFewKeys * rows);
+  }
 
   // Sequence b: its rows, its keys in order of position without the hidden
   // ones between the sinks and the window of its first new token, and its
@@ -121,7 +133,7 @@ struct AttWork {
     s.head = min(sinks, s.start);
     s.keys = s.len - s.start + s.head;
     s.row_tiles = (static_cast<uint32_t>(s.count) * group + row_tile - 1) / row_tile;
-    s.tiles = s.count > 0 && s.count * group <= most_rows
+    s.tiles = s.count > 0 && (!shared || few(s.count * group, s.len))
                   ? max(1, (s.keys + kAttKeys - 1) / kAttKeys)
                   : 0u;
     return s;
@@ -131,18 +143,20 @@ struct AttWork {
   }
 };
 
-// Exclusive prefix sums of the sequences' units by blocks of 32 * kAttWarps
-// consecutive ones. find() leaves, in shared memory, the sequence that holds
-// unit u and its first unit; total() the number of units.
+// Exclusive prefix sums of the sequences' units, a run of sequences per thread
+// of the CTA's W warps. att_find leaves the sequence that holds unit u and its
+// first unit.
+template <int W>
 struct AttScan {
-  uint64_t part[32 * kAttWarps];  // units before thread i's sequences
-  uint64_t sums[kAttWarps];       // of the warps
+  uint64_t part[32 * W];  // units before thread i's sequences
+  uint64_t sums[W];       // of the warps
   uint64_t total, before;
   uint32_t seq;
 };
 
-__device__ __forceinline__ void att_scan(const AttWork& w, AttScan& sc) {
-  const uint32_t per = (w.kv.batch + 32 * kAttWarps - 1) / (32 * kAttWarps);
+template <int W>
+__device__ __forceinline__ void att_scan(const AttWork& w, AttScan<W>& sc) {
+  const uint32_t per = (w.kv.batch + 32 * W - 1) / (32 * W);
   const uint32_t b0 = threadIdx.x * per, b1 = min(w.kv.batch, b0 + per);
   uint64_t n = 0;
   for (uint32_t b = b0; b < b1; ++b) n += w.units(w.seq(b));
@@ -157,7 +171,7 @@ __device__ __forceinline__ void att_scan(const AttWork& w, AttScan& sc) {
   __syncthreads();
   uint64_t base = 0, all = 0;
 #pragma unroll
-  for (int i = 0; i < kAttWarps; ++i) {
+  for (int i = 0; i < W; ++i) {
     if (i < warp) base += sc.sums[i];
     all += sc.sums[i];
   }
@@ -167,10 +181,11 @@ __device__ __forceinline__ void att_scan(const AttWork& w, AttScan& sc) {
 }
 
 // After att_scan: the sequence that holds unit u (< total) and the units before it.
-__device__ __forceinline__ void att_find(const AttWork& w, AttScan& sc, uint64_t u) {
-  const uint32_t per = (w.kv.batch + 32 * kAttWarps - 1) / (32 * kAttWarps);
+template <int W>
+__device__ __forceinline__ void att_find(const AttWork& w, AttScan<W>& sc, uint64_t u) {
+  const uint32_t per = (w.kv.batch + 32 * W - 1) / (32 * W);
   const uint64_t lo = sc.part[threadIdx.x];
-  const uint64_t hi = threadIdx.x + 1 < 32 * kAttWarps ? sc.part[threadIdx.x + 1] : sc.total;
+  const uint64_t hi = threadIdx.x + 1 < 32 * W ? sc.part[threadIdx.x + 1] : sc.total;
   if (u >= lo && u < hi) {
     uint64_t at = lo;
     uint32_t b = threadIdx.x * per;
@@ -210,7 +225,8 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
   using L = AttLayout<D>;
   constexpr int NR = 8 * NT, KS = D / 16;
   extern __shared__ __align__(128) uint8_t smem[];
-  AttScan& sc = *reinterpret_cast<AttScan*>(smem + L::kRing);  // read before the first merge
+  AttScan<kAttWarps>& sc =
+      *reinterpret_cast<AttScan<kAttWarps>*>(smem + L::kRing);  // read before the first merge
   __shared__ float s_m[kAttWarps][NR], s_f[kAttWarps][NR], s_top[NR];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
@@ -514,88 +530,94 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
   cp_async_wait<0>();
 }
 
-// Joins the parts of each row tile whose keys were split. One CTA per row
-// (blockIdx.x = row of kv head's row tiles, blockIdx.y = sequence, in strides):
-// the parts' factors first, then their outputs, a thread per dimension.
+// Joins the parts of the row tiles whose keys were split: CTA c the row tile
+// that CTA c of the first kernel began and the next one went on with. A warp
+// per row: the parts' factors, a part a lane, then their outputs, D / 32
+// dimensions a lane.
+constexpr int kJoinWarps = 8;
+
 template <int DT, int D, int NR>
-__global__ void __launch_bounds__(32 * kAttWarps)
+__global__ void __launch_bounds__(32 * kJoinWarps)
     attention_join_kernel(char* out, const AttWork w, int64_t ld_o, uint32_t launched,
                           const float* __restrict__ ws) {
-  using T = typename DType<DT>::T;
-  constexpr int kThreads = 32 * kAttWarps, kSets = kThreads / D;
-  __shared__ AttScan sc;
-  __shared__ float s_f[kAttMaxCtas], s_red[kAttWarps], s_v[kThreads];
+  constexpr int E = D / 32;
+  __shared__ AttScan<kJoinWarps> sc;
+  __shared__ float s_f[kJoinWarps][kAttMaxCtas];
   // The lengths are older than the first kernel, which let this one start.
   att_scan(w, sc);
   const uint64_t total = sc.total;
-  const uint32_t ctas = att_ctas(total, launched);
+  const uint32_t ctas = att_ctas(total, launched), c0 = blockIdx.x;
   pdl_launch_dependents();
+  if (c0 + 1 >= ctas) {
+    pdl_wait();
+    return;
+  }
+  const uint64_t u0 = att_first_unit(total, c0, ctas), u1 = att_first_unit(total, c0 + 1, ctas);
+  att_find(w, sc, u1);
+  const AttWork::Seq s = w.seq(sc.seq);
+  const uint32_t per = s.tiles + kAttRowCost;
+  const uint32_t hr = static_cast<uint32_t>((u1 - sc.before) / per);
+  // units before the row tile, of its first and of its last key tile
+  const uint64_t begin = sc.before + static_cast<uint64_t>(hr) * per, f = begin + kAttRowCost;
+  const uint64_t e = begin + per - 1;
   pdl_wait();
-  const uint32_t per = (w.kv.batch + kThreads - 1) / kThreads;
-  for (uint32_t b = blockIdx.y; b < w.kv.batch; b += gridDim.y) {
-    const AttWork::Seq s = w.seq(b);
-    if (s.tiles < 2) continue;
-    uint64_t before = sc.part[b / per];
-    for (uint32_t i = b / per * per; i < b; ++i) before += w.units(w.seq(i));
-    for (uint32_t x = blockIdx.x; x < s.row_tiles * w.kv.n_kv * NR; x += gridDim.x) {
-      const uint32_t hr = x / NR, r = x % NR;
-      const uint32_t hk = hr / s.row_tiles, row = (hr - hk * s.row_tiles) * NR + r;
-      if (row >= s.count * w.group) continue;
-      // units of its first and its last key tile
-      const uint64_t f = before + static_cast<uint64_t>(hr) * (s.tiles + kAttRowCost) + kAttRowCost;
-      const uint64_t e = f + s.tiles - 1;
-      auto owner = [&](uint64_t u) {
-        uint32_t c = static_cast<uint32_t>(u * ctas / total);
-        while (att_first_unit(total, c + 1, ctas) <= u) ++c;
-        return c;
-      };
-      const uint32_t c0 = owner(f), parts = owner(e) - c0 + 1;
-      if (parts == 1) continue;  // written whole by its CTA
-      // whether that CTA worked on another row tile before
-      const bool late = att_first_unit(total, c0, ctas) < f - kAttRowCost;
-      auto slot = [&](uint32_t i) {
-        return ws + static_cast<size_t>(2 * (c0 + i) + (i == 0 && late)) * NR * (D + 2);
-      };
-      float top = -INFINITY;
-      for (uint32_t i = threadIdx.x; i < parts; i += kThreads) {
-        const float m = slot(i)[r];
-        s_f[i] = m;
-        top = fmaxf(top, m);
-      }
-      top = block_reduce<true>(top, s_red);
-      const float base = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
-      for (uint32_t i = threadIdx.x; i < parts; i += kThreads) {
-        const float k = exp2_approx(s_f[i] - base);
-        s_f[i] = k;
-        sum += slot(i)[NR + r] * k;
-      }
-      sum = block_reduce<false>(sum, s_red);  // (its barriers publish s_f too)
-      const int c = threadIdx.x % D;
-      float v = 0.f;
-#pragma unroll 8
-      for (uint32_t i = threadIdx.x / D; i < parts; i += kSets)
-        v += slot(i)[2 * NR + r * D + c] * s_f[i];
-      if constexpr (kSets > 1) {
-        s_v[threadIdx.x] = v;
-        __syncthreads();
-        for (int k = 1; k < kSets; ++k) v += s_v[(threadIdx.x + k * D) % kThreads];
-      }
-      if (threadIdx.x < D) {
-        const uint32_t tok = w.by_group.div(row);
-        T* dst = reinterpret_cast<T*>(out + (s.first + tok) * ld_o +
-                                      static_cast<int64_t>(hk * w.group + row - tok * w.group) * (2 * D));
-        dst[c] = DType<DT>::from_f32(sum != 0.f ? v / sum : 0.f);
-      }
-      __syncthreads();  // s_f and s_v are written again
+  if (f >= u1 || f < u0) return;  // not split here, or begun by an earlier CTA
+  uint32_t c1 = static_cast<uint32_t>(e * ctas / total);
+  while (att_first_unit(total, c1 + 1, ctas) <= e) ++c1;
+  const uint32_t parts = c1 - c0 + 1;
+  const bool late = u0 < begin;  // that CTA worked on another row tile before
+  const uint32_t hk = hr / s.row_tiles, r0 = (hr - hk * s.row_tiles) * NR;
+  const int rows = min(NR, static_cast<int>(s.count * w.group - r0));
+  auto slot = [&](uint32_t i) {
+    return ws + static_cast<size_t>(2 * (c0 + i) + (i == 0 && late)) * NR * (D + 2);
+  };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = warp; r < rows; r += kJoinWarps) {
+    float top = -INFINITY;
+    for (uint32_t i = lane; i < parts; i += 32) {
+      const float m = slot(i)[r];
+      s_f[warp][i] = m;
+      top = fmaxf(top, m);
     }
+    top = warp_reduce<true>(top);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    for (uint32_t i = lane; i < parts; i += 32) {
+      const float k = exp2_approx(s_f[warp][i] - base);
+      s_f[warp][i] = k;
+      sum += slot(i)[NR + r] * k;
+    }
+    sum = warp_reduce<false>(sum);
+    __syncwarp();
+    float v[E] = {};
+#pragma unroll 8
+    for (uint32_t i = 0; i < parts; ++i) {
+      const float* p = slot(i) + 2 * NR + r * D + E * lane;
+      const float k = s_f[warp][i];
+      if constexpr (E == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        v[0] += x.x * k, v[1] += x.y * k, v[2] += x.z * k, v[3] += x.w * k;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(p);
+        v[0] += x.x * k, v[1] += x.y * k;
+      }
+    }
+    __syncwarp();  // s_f is written again
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    const uint32_t row = r0 + r, tok = w.by_group.div(row);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(
+        out + (s.first + tok) * ld_o +
+        static_cast<int64_t>(hk * w.group + row - tok * w.group) * (2 * D) + 2 * E * lane);
+#pragma unroll
+    for (int k = 0; k < E; k += 2)
+      dst[k / 2] = sum != 0.f ? pack2<DT>(v[k] * inv, v[k + 1] * inv) : 0u;
   }
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
 
 inline AttWork att_work(const AttentionProblem& p, const PagedView& kv, uint32_t row_tile,
-                        uint32_t most_rows = 0xffffffffu) {
+                        bool shared) {
   AttWork w;
   w.kv = kv;
   w.tokens = static_cast<uint32_t>(p.tokens);
@@ -604,7 +626,7 @@ inline AttWork att_work(const AttentionProblem& p, const PagedView& kv, uint32_t
   w.by_group = FastDiv(w.group);
   w.window = p.window;
   w.sinks = p.sinks;
-  w.most_rows = most_rows;
+  w.shared = shared;
   return w;
 }
 
@@ -619,12 +641,12 @@ inline uint64_t att_most_units(size_t batch, size_t tokens, size_t group, size_t
 
 template <int DT, int D, int NT, bool MULTI>
 cudaError_t launch_attention_split_t(const AttentionProblem& p, const PagedView& kv,
-                                     uint32_t most_rows) {
+                                     bool shared) {
   static uint64_t done = 0;  // a lost update only repeats the call
   auto kern = attention_split_kernel<DT, D, NT, MULTI>;
   cudaError_t e = allow_smem(kern, AttLayout<D>::kSmem, p.device, &done);
   if (e != cudaSuccess) return e;
-  AttWork w = att_work(p, kv, 8 * NT, most_rows);
+  AttWork w = att_work(p, kv, 8 * NT, shared);
   const size_t keys = static_cast<size_t>(kv.width) * kv.page.d;
   const uint64_t most = att_most_units(kv.batch, p.tokens, w.group, kv.n_kv, keys, 8 * NT, MULTI);
   uint32_t ctas = static_cast<uint32_t>(
@@ -638,14 +660,10 @@ cudaError_t launch_attention_split_t(const AttentionProblem& p, const PagedView&
   e = launch_pdl(kern, dim3(ctas), 32 * kAttWarps, AttLayout<D>::kSmem, p.stream, a);
   // no row tile can be split: its keys fit one unit
   if (e != cudaSuccess || keys <= kAttKeys || ctas == 1) return e;
-  const uint64_t rows = static_cast<uint64_t>(kv.n_kv) * 8 * NT *
-                        ((w.group * (MULTI ? (p.tokens + kv.batch - 1) / kv.batch : 1) + 8 * NT - 1) / (8 * NT));
   const float* cws = ws;
   void* b[] = {&out, &w, &ld_o, &ctas, &cws};
-  return launch_pdl(attention_join_kernel<DT, D, 8 * NT>,
-                    dim3(static_cast<uint32_t>(std::min<uint64_t>(rows, 4096)),
-                         std::min<uint32_t>(kv.batch, 65535)),
-                    32 * kAttWarps, 0, p.stream, b);
+  return launch_pdl(attention_join_kernel<DT, D, 8 * NT>, dim3(ctas - 1), 32 * kJoinWarps, 0,
+                    p.stream, b);
 }
 
 inline size_t att_row_tile(size_t group, bool multi) { return multi || group > 8 ? 16 : 8; }
@@ -658,13 +676,13 @@ inline size_t attention_split_workspace(size_t batch, size_t tokens, size_t grou
 }
 
 cudaError_t launch_attention_split(const AttentionProblem& p, const PagedView& kv,
-                                   uint32_t most_rows = 0xffffffffu) {
+                                   bool shared) {
   const bool multi = kv.q_start != nullptr;
   const bool two = att_row_tile(p.n_q / kv.n_kv, multi) == 16;
 #define CAWQ_ATT(DT, D)                                                    \
-  (multi ? launch_attention_split_t<DT, D, 2, true>(p, kv, most_rows)                 \
-         : two ? launch_attention_split_t<DT, D, 2, false>(p, kv, most_rows)          \
-               : launch_attention_split_t<DT, D, 1, false>(p, kv, most_rows))
+  (multi ? launch_attention_split_t<DT, D, 2, true>(p, kv, shared)                 \
+         : two ? launch_attention_split_t<DT, D, 2, false>(p, kv, shared)          \
+               : launch_attention_split_t<DT, D, 1, false>(p, kv, shared))
   if (p.dtype == kF16) return p.d == 64 ? CAWQ_ATT(kF16, 64) : CAWQ_ATT(kF16, 128);
   return p.d == 64 ? CAWQ_ATT(kBF16, 64) : CAWQ_ATT(kBF16, 128);
 #undef CAWQ_ATT

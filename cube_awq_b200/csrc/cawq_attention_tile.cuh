@@ -119,7 +119,6 @@ struct TileArgs {
   int64_t ld_q, ld_o;
   float scale_log2;   // > 0
   uint32_t negate;    // the score product's "negate A" bit with a negative scale
-  uint32_t least;     // sequences with fewer rows belong to the split kernel
   uint32_t box;       // keys of a TMA box: divides page size and 128, a multiple of 8
   int64_t heads_per_page;  // page stride / head stride
 };
@@ -197,7 +196,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       w.kv.rows(b, w.tokens, first, count);
       *len = w.kv.len(b);
       const uint32_t rows = static_cast<uint32_t>(*count) * w.group;
-      return rows >= a.least ? (rows + kTileRows - 1) / kTileRows : 0u;
+      return w.shared && AttWork::few(rows, *len) ? 0u : (rows + kTileRows - 1) / kTileRows;
     };
     const uint32_t per = (w.kv.batch + kTileThreads - 1) / kTileThreads;
     const uint32_t b0 = min(w.kv.batch, tid * per), b1 = min(w.kv.batch, b0 + per);
@@ -673,7 +672,7 @@ inline bool encode_cache(CUtensorMap* map, int dtype, const void* base, const Pa
 }
 
 template <int DT, int D>
-cudaError_t launch_attention_tile_t(const AttentionProblem& p, const PagedView& kv, uint32_t least) {
+cudaError_t launch_attention_tile_t(const AttentionProblem& p, const PagedView& kv, bool shared) {
   static uint64_t done = 0;
   auto kern = attention_tile_kernel<DT, D>;
   cudaError_t e = allow_smem(kern, TileLayout<D>::kSmem, p.device, &done);
@@ -681,13 +680,12 @@ cudaError_t launch_attention_tile_t(const AttentionProblem& p, const PagedView& 
   TileArgs a;
   a.q = static_cast<const char*>(p.q);
   a.out = static_cast<char*>(p.out);
-  a.w = att_work(p, kv, 0);
+  a.w = att_work(p, kv, 0, shared);
   a.ld_q = static_cast<int64_t>(p.ld_q) * 2;
   a.ld_o = static_cast<int64_t>(p.ld_out) * 2;
   // scores of a scale of 0 are all equal: so they are at 1e-30
   a.scale_log2 = std::max(std::abs(p.scale) * kLog2e, 1e-30f);
   a.negate = p.scale < 0 ? 1u << 13 : 0u;
-  a.least = least;
   a.box = 8;
   while (a.box < kTileKeys && kv.page.d % (2 * a.box) == 0) a.box *= 2;
   a.heads_per_page = static_cast<int64_t>(tile_heads_per_page(kv));
@@ -700,12 +698,12 @@ cudaError_t launch_attention_tile_t(const AttentionProblem& p, const PagedView& 
                     TileLayout<D>::kSmem, p.stream, args);
 }
 
-cudaError_t launch_attention_tile(const AttentionProblem& p, const PagedView& kv, uint32_t least) {
+cudaError_t launch_attention_tile(const AttentionProblem& p, const PagedView& kv, bool shared) {
   if (p.dtype == kF16)
-    return p.d == 64 ? launch_attention_tile_t<kF16, 64>(p, kv, least)
-                     : launch_attention_tile_t<kF16, 128>(p, kv, least);
-  return p.d == 64 ? launch_attention_tile_t<kBF16, 64>(p, kv, least)
-                   : launch_attention_tile_t<kBF16, 128>(p, kv, least);
+    return p.d == 64 ? launch_attention_tile_t<kF16, 64>(p, kv, shared)
+                     : launch_attention_tile_t<kF16, 128>(p, kv, shared);
+  return p.d == 64 ? launch_attention_tile_t<kBF16, 64>(p, kv, shared)
+                   : launch_attention_tile_t<kBF16, 128>(p, kv, shared);
 }
 
 }  // namespace cawq

@@ -201,12 +201,15 @@ static cawq_status attention(const void* q, void* out, const cawq_paged_kv* kv, 
                               static_cast<int>(std::min(sinks, kMaxInt)), dtype, workspace,
                               dev.sm_count, dev.device, static_cast<cudaStream_t>(stream)};
   const PagedView view = paged_view(*kv, 2, decode);
-  cudaError_t e;
-  if (decode || tile_heads_per_page(view) == 0) {
-    e = launch_attention_split(p, view);
-  } else {
-    e = launch_attention_tile(p, view, 0);
-  }
+  // Sequences with few query rows go to the split kernel, the others to the
+  // tile kernel (AttWork::few). Where the host knows that all are of one kind,
+  // one kernel runs; otherwise both, each on its own sequences.
+  const size_t rows = tokens * (n_q / kv->n_kv);  // of a kv head, in all
+  const bool tile = !decode && rows > kAttFew && tile_heads_per_page(view) != 0;
+  const bool split = !tile || kv->batch > 1 || rows <= kAttFewLong;
+  cudaError_t e = cudaSuccess;
+  if (tile) e = launch_attention_tile(p, view, split);
+  if (split && e == cudaSuccess) e = launch_attention_split(p, view, tile);
   return e == cudaSuccess ? CAWQ_OK : cuda_fail(e, "attention launch");
 }
 
