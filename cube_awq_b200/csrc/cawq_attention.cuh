@@ -43,9 +43,10 @@ constexpr int kAttStages = 3;
 // long ones left the CTAs with the short ones last (64 sequences of 1 to 8000
 // tokens, 28 / 4 heads: 62 us).
 constexpr uint32_t kAttRowCost = 2;
-// Query rows of a (sequence, kv head) that are few: always up to the first
-// number; up to the second if there are that many keys to a row to split.
-constexpr uint32_t kAttFew = 16, kAttFewLong = 128, kAttFewKeys = 40;
+// A sequence is for the split kernel rather than the tile kernel with no more
+// query rows (of a kv head) than the first number, no fewer keys than the
+// second and than the third times its rows.
+constexpr uint32_t kAttFewRows = 128, kAttFewKeys = 1024, kAttFewPerRow = 40;
 constexpr int kAttMaxCtas = 320;  // most CTAs of a launch (two per SM)
 
 template <int D>
@@ -106,13 +107,14 @@ struct AttWork {
   int window, sinks;
   bool shared;  // the tile kernel takes the sequences whose rows are not few
 
-  // Few rows are bound by their keys' bytes and gain from the split; many by
-  // the tensor cores. Per call, us split / tiles (D = 128, bf16, one
-  // sequence): 64 rows, 8 kv heads at 500 / 3000 / 20000 keys 22 / 31 / 101
-  // against 11 / 35 / 187; 128 rows 25 / 45 / 181 against 12 / 35 / 188.
-  __device__ __forceinline__ static bool few(uint32_t rows, int len) {
-    return rows <= kAttFew ||
-           (rows <= kAttFewLong && static_cast<uint32_t>(len) >= kAttFewKeys * rows);
+  // Few rows are bound by their keys' bytes and gain from the split; many, or
+  // few keys, do as well in a tile. Per call, us split / tiles (D = 128, bf16,
+  // one sequence): 16 rows, 8 kv heads at 500 / 3000 / 20000 keys 11 / 23 / 41
+  // against 11 / 34 / 186; 64 rows 22 / 31 / 101 against 11 / 35 / 187; 128
+  // rows 25 / 45 / 181 against 12 / 35 / 188.
+  __host__ __device__ __forceinline__ static bool few(uint32_t rows, int len) {
+    const uint32_t n = static_cast<uint32_t>(len);
+    return rows <= kAttFewRows && n >= kAttFewKeys && n >= kAttFewPerRow * rows;
   }
 
   // Sequence b: its rows, its keys in order of position without the hidden
@@ -144,18 +146,18 @@ struct AttWork {
 };
 
 // Exclusive prefix sums of the sequences' units, a run of sequences per thread
-// of the CTA's W warps. att_find leaves the sequence that holds unit u and its
+// of the CTA. att_find leaves the sequence that holds unit u and its
 // first unit.
-template <int W>
 struct AttScan {
+  static constexpr int W = kAttWarps;
   uint64_t part[32 * W];  // units before thread i's sequences
   uint64_t sums[W];       // of the warps
   uint64_t total, before;
   uint32_t seq;
 };
 
-template <int W>
-__device__ __forceinline__ void att_scan(const AttWork& w, AttScan<W>& sc) {
+__device__ __forceinline__ void att_scan(const AttWork& w, AttScan& sc) {
+  constexpr int W = kAttWarps;
   const uint32_t per = (w.kv.batch + 32 * W - 1) / (32 * W);
   const uint32_t b0 = threadIdx.x * per, b1 = min(w.kv.batch, b0 + per);
   uint64_t n = 0;
@@ -181,8 +183,8 @@ __device__ __forceinline__ void att_scan(const AttWork& w, AttScan<W>& sc) {
 }
 
 // After att_scan: the sequence that holds unit u (< total) and the units before it.
-template <int W>
-__device__ __forceinline__ void att_find(const AttWork& w, AttScan<W>& sc, uint64_t u) {
+__device__ __forceinline__ void att_find(const AttWork& w, AttScan& sc, uint64_t u) {
+  constexpr int W = kAttWarps;
   const uint32_t per = (w.kv.batch + 32 * W - 1) / (32 * W);
   const uint64_t lo = sc.part[threadIdx.x];
   const uint64_t hi = threadIdx.x + 1 < 32 * W ? sc.part[threadIdx.x + 1] : sc.total;
@@ -209,10 +211,22 @@ __device__ __forceinline__ uint64_t att_first_unit(uint64_t total, uint32_t cta,
   return total * cta / ctas;
 }
 
+// The workspace begins with a note of each CTA on the row tile that it began
+// and left to the next ones (parts = 0: none), for the joining kernel.
+struct AttNote {
+  uint32_t parts;  // parts of the row tile; that CTA's first
+  uint32_t late;   // that CTA worked on another row tile before
+  int first;       // row of q of the sequence's first token
+  uint32_t hk, r0;
+  int rows;
+  uint32_t pad[2];
+};
+constexpr size_t kAttNotes = kAttMaxCtas * sizeof(AttNote);
+
 // A part in the workspace: NR maxima, NR sums, NR x D outputs.
 template <int D, int NR>
-__device__ __forceinline__ float* att_slot(float* ws, uint32_t slot) {
-  return ws + static_cast<size_t>(slot) * NR * (D + 2);
+__device__ __forceinline__ float* att_slot(char* ws, uint32_t slot) {
+  return reinterpret_cast<float*>(ws + kAttNotes) + static_cast<size_t>(slot) * NR * (D + 2);
 }
 
 // MULTI: sequences may have several new tokens, so rows of a tile see
@@ -220,13 +234,12 @@ __device__ __forceinline__ float* att_slot(float* ws, uint32_t slot) {
 template <int DT, int D, int NT, bool MULTI>
 __global__ void __launch_bounds__(32 * kAttWarps, 2)
     attention_split_kernel(const char* q, char* out, const AttWork w, int64_t ld_q, int64_t ld_o,
-                           float scale_log2, float* ws) {
+                           float scale_log2, char* ws) {
   using T = typename DType<DT>::T;
   using L = AttLayout<D>;
   constexpr int NR = 8 * NT, KS = D / 16;
   extern __shared__ __align__(128) uint8_t smem[];
-  AttScan<kAttWarps>& sc =
-      *reinterpret_cast<AttScan<kAttWarps>*>(smem + L::kRing);  // read before the first merge
+  AttScan& sc = *reinterpret_cast<AttScan*>(smem + L::kRing);  // read before the first merge
   __shared__ float s_m[kAttWarps][NR], s_f[kAttWarps][NR], s_top[NR];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
@@ -234,10 +247,13 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
   pdl_wait();
   pdl_launch_dependents();  // after the wait: the joining kernel may read the lengths at once
   att_scan(w, sc);
-  const uint32_t ctas = att_ctas(sc.total, gridDim.x);
+  const uint64_t total = sc.total;
+  const uint32_t ctas = att_ctas(total, gridDim.x);
+  AttNote* note = reinterpret_cast<AttNote*>(ws) + blockIdx.x;
+  if (threadIdx.x == 0) note->parts = 0;
   if (blockIdx.x >= ctas) return;
-  const uint64_t u0 = att_first_unit(sc.total, blockIdx.x, ctas);
-  const uint64_t u1 = att_first_unit(sc.total, blockIdx.x + 1, ctas);
+  const uint64_t u0 = att_first_unit(total, blockIdx.x, ctas);
+  const uint64_t u1 = att_first_unit(total, blockIdx.x + 1, ctas);
   att_find(w, sc, u0);
 
   // ---- the stream of 64-key tiles: a cursor that runs ahead of the work
@@ -477,6 +493,13 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
     const uint32_t r0 = (done.hr - hk * done.s.row_tiles) * NR;
     const int rows = min(NR, static_cast<int>(done.s.count * w.group - r0));
     float* part = att_slot<D, NR>(ws, 2 * blockIdx.x + (first_rows ? 0 : 1));
+    if (!go_on && tile0 == 0 && !whole && threadIdx.x == 0) {
+      // the last key tile's unit is this many on from the CTA's end
+      const uint64_t e = u1 - 1 + (done.s.tiles - 1 - done.tile);
+      uint32_t c1 = static_cast<uint32_t>(e * ctas / total);
+      while (att_first_unit(total, c1 + 1, ctas) <= e) ++c1;
+      *note = {c1 - blockIdx.x + 1, first_rows ? 0u : 1u, done.s.first, hk, r0, rows, {0, 0}};
+    }
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
 #pragma unroll
@@ -530,70 +553,46 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
   cp_async_wait<0>();
 }
 
-// Joins the parts of the row tiles whose keys were split: CTA c the row tile
-// that CTA c of the first kernel began and the next one went on with. A warp
-// per row: the parts' factors, a part a lane, then their outputs, D / 32
-// dimensions a lane.
-constexpr int kJoinWarps = 8;
+// Joins the parts of the row tiles whose keys were split: blockIdx.x is the CTA
+// that began one, blockIdx.y deals out its rows. The parts' factors first, then
+// their outputs: a warp takes every eighth part, a lane D / 32 dimensions.
+constexpr int kJoinWarps = 8, kJoinRows = 8;
 
 template <int DT, int D, int NR>
 __global__ void __launch_bounds__(32 * kJoinWarps)
-    attention_join_kernel(char* out, const AttWork w, int64_t ld_o, uint32_t launched,
-                          const float* __restrict__ ws) {
-  constexpr int E = D / 32;
-  __shared__ AttScan<kJoinWarps> sc;
-  __shared__ float s_f[kJoinWarps][kAttMaxCtas];
-  // The lengths are older than the first kernel, which let this one start.
-  att_scan(w, sc);
-  const uint64_t total = sc.total;
-  const uint32_t ctas = att_ctas(total, launched), c0 = blockIdx.x;
+    attention_join_kernel(char* out, const FastDiv by_group, int64_t ld_o, char* ws) {
+  using T = typename DType<DT>::T;
+  constexpr int E = D / 32, kThreads = 32 * kJoinWarps;
+  __shared__ float s_f[kAttMaxCtas], s_red[kJoinWarps], s_v[kJoinWarps][D];
   pdl_launch_dependents();
-  if (c0 + 1 >= ctas) {
-    pdl_wait();
-    return;
-  }
-  const uint64_t u0 = att_first_unit(total, c0, ctas), u1 = att_first_unit(total, c0 + 1, ctas);
-  att_find(w, sc, u1);
-  const AttWork::Seq s = w.seq(sc.seq);
-  const uint32_t per = s.tiles + kAttRowCost;
-  const uint32_t hr = static_cast<uint32_t>((u1 - sc.before) / per);
-  // units before the row tile, of its first and of its last key tile
-  const uint64_t begin = sc.before + static_cast<uint64_t>(hr) * per, f = begin + kAttRowCost;
-  const uint64_t e = begin + per - 1;
   pdl_wait();
-  if (f >= u1 || f < u0) return;  // not split here, or begun by an earlier CTA
-  uint32_t c1 = static_cast<uint32_t>(e * ctas / total);
-  while (att_first_unit(total, c1 + 1, ctas) <= e) ++c1;
-  const uint32_t parts = c1 - c0 + 1;
-  const bool late = u0 < begin;  // that CTA worked on another row tile before
-  const uint32_t hk = hr / s.row_tiles, r0 = (hr - hk * s.row_tiles) * NR;
-  const int rows = min(NR, static_cast<int>(s.count * w.group - r0));
-  auto slot = [&](uint32_t i) {
-    return ws + static_cast<size_t>(2 * (c0 + i) + (i == 0 && late)) * NR * (D + 2);
-  };
+  const AttNote note = reinterpret_cast<const AttNote*>(ws)[blockIdx.x];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int r = warp; r < rows; r += kJoinWarps) {
+  auto slot = [&](uint32_t i) {
+    return att_slot<D, NR>(ws, 2 * (blockIdx.x + i) + (i == 0 ? note.late : 0u));
+  };
+  if (note.parts == 0) return;
+  for (int r = blockIdx.y; r < note.rows; r += kJoinRows) {
     float top = -INFINITY;
-    for (uint32_t i = lane; i < parts; i += 32) {
+    for (uint32_t i = threadIdx.x; i < note.parts; i += kThreads) {
       const float m = slot(i)[r];
-      s_f[warp][i] = m;
+      s_f[i] = m;
       top = fmaxf(top, m);
     }
-    top = warp_reduce<true>(top);
+    top = block_reduce<true>(top, s_red);
     const float base = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
-    for (uint32_t i = lane; i < parts; i += 32) {
-      const float k = exp2_approx(s_f[warp][i] - base);
-      s_f[warp][i] = k;
+    for (uint32_t i = threadIdx.x; i < note.parts; i += kThreads) {
+      const float k = exp2_approx(s_f[i] - base);
+      s_f[i] = k;
       sum += slot(i)[NR + r] * k;
     }
-    sum = warp_reduce<false>(sum);
-    __syncwarp();
+    sum = block_reduce<false>(sum, s_red);  // (its barriers publish s_f too)
     float v[E] = {};
-#pragma unroll 8
-    for (uint32_t i = 0; i < parts; ++i) {
+#pragma unroll 4
+    for (uint32_t i = warp; i < note.parts; i += kJoinWarps) {
       const float* p = slot(i) + 2 * NR + r * D + E * lane;
-      const float k = s_f[warp][i];
+      const float k = s_f[i];
       if constexpr (E == 4) {
         const float4 x = *reinterpret_cast<const float4*>(p);
         v[0] += x.x * k, v[1] += x.y * k, v[2] += x.z * k, v[3] += x.w * k;
@@ -602,15 +601,19 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
         v[0] += x.x * k, v[1] += x.y * k;
       }
     }
-    __syncwarp();  // s_f is written again
-    const float inv = sum != 0.f ? 1.f / sum : 0.f;
-    const uint32_t row = r0 + r, tok = w.by_group.div(row);
-    uint32_t* dst = reinterpret_cast<uint32_t*>(
-        out + (s.first + tok) * ld_o +
-        static_cast<int64_t>(hk * w.group + row - tok * w.group) * (2 * D) + 2 * E * lane);
 #pragma unroll
-    for (int k = 0; k < E; k += 2)
-      dst[k / 2] = sum != 0.f ? pack2<DT>(v[k] * inv, v[k + 1] * inv) : 0u;
+    for (int k = 0; k < E; ++k) s_v[warp][E * lane + k] = v[k];
+    __syncthreads();
+    if (threadIdx.x < D) {
+      float o = 0.f;
+#pragma unroll
+      for (int k = 0; k < kJoinWarps; ++k) o += s_v[k][threadIdx.x];
+      const uint32_t row = note.r0 + r, tok = by_group.div(row), group = by_group.d;
+      T* dst = reinterpret_cast<T*>(out + (note.first + tok) * ld_o +
+                                    static_cast<int64_t>(note.hk * group + row - tok * group) * (2 * D));
+      dst[threadIdx.x] = DType<DT>::from_f32(sum != 0.f ? o / sum : 0.f);
+    }
+    __syncthreads();  // s_f and s_v are written again
   }
 }
 
@@ -655,15 +658,15 @@ cudaError_t launch_attention_split_t(const AttentionProblem& p, const PagedView&
   char* out = static_cast<char*>(p.out);
   int64_t ld_q = static_cast<int64_t>(p.ld_q) * 2, ld_o = static_cast<int64_t>(p.ld_out) * 2;
   float sl = p.scale * kLog2e;
-  float* ws = static_cast<float*>(p.workspace);
+  char* ws = static_cast<char*>(p.workspace);
   void* a[] = {&q, &out, &w, &ld_q, &ld_o, &sl, &ws};
   e = launch_pdl(kern, dim3(ctas), 32 * kAttWarps, AttLayout<D>::kSmem, p.stream, a);
   // no row tile can be split: its keys fit one unit
   if (e != cudaSuccess || keys <= kAttKeys || ctas == 1) return e;
-  const float* cws = ws;
-  void* b[] = {&out, &w, &ld_o, &ctas, &cws};
-  return launch_pdl(attention_join_kernel<DT, D, 8 * NT>, dim3(ctas - 1), 32 * kJoinWarps, 0,
-                    p.stream, b);
+  FastDiv by_group = w.by_group;
+  void* b[] = {&out, &by_group, &ld_o, &ws};
+  return launch_pdl(attention_join_kernel<DT, D, 8 * NT>, dim3(ctas - 1, kJoinRows),
+                    32 * kJoinWarps, 0, p.stream, b);
 }
 
 inline size_t att_row_tile(size_t group, bool multi) { return multi || group > 8 ? 16 : 8; }
@@ -672,7 +675,7 @@ inline size_t attention_split_workspace(size_t batch, size_t tokens, size_t grou
                                         size_t keys, size_t d, bool multi) {
   const size_t nr = att_row_tile(group, multi);
   const uint64_t most = att_most_units(batch, tokens, group, n_kv, keys, nr, multi);
-  return std::min<uint64_t>(most, kAttMaxCtas) * 2 * nr * (d + 2) * sizeof(float);
+  return kAttNotes + std::min<uint64_t>(most, kAttMaxCtas) * 2 * nr * (d + 2) * sizeof(float);
 }
 
 cudaError_t launch_attention_split(const AttentionProblem& p, const PagedView& kv,

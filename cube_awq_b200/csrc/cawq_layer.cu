@@ -201,12 +201,22 @@ static cawq_status attention(const void* q, void* out, const cawq_paged_kv* kv, 
                               static_cast<int>(std::min(sinks, kMaxInt)), dtype, workspace,
                               dev.sm_count, dev.device, static_cast<cudaStream_t>(stream)};
   const PagedView view = paged_view(*kv, 2, decode);
-  // Sequences with few query rows go to the split kernel, the others to the
-  // tile kernel (AttWork::few). Where the host knows that all are of one kind,
-  // one kernel runs; otherwise both, each on its own sequences.
+  // Long sequences with few query rows go to the split kernel, the others to
+  // the tile kernel (AttWork::few). The lengths are the device's; the host goes
+  // by what it knows, the rows in all and what the table can hold: one kernel
+  // for one sequence, for few rows in all, for short tables and for batches of
+  // prompts (1024 rows a sequence and more); else both, each on its own
+  // sequences (an empty one costs about 10 us: the second of a batch of prompts
+  // took it from 95 to 124 us).
   const size_t rows = tokens * (n_q / kv->n_kv);  // of a kv head, in all
-  const bool tile = !decode && rows > kAttFew && tile_heads_per_page(view) != 0;
-  const bool split = !tile || kv->batch > 1 || rows <= kAttFewLong;
+  const size_t room = kv->table_width * kv->page_size;
+  bool split = decode || tile_heads_per_page(view) == 0, tile = !split;
+  if (tile && (rows <= kAttFewRows || (kv->batch > 1 && rows < 1024 * kv->batch))) {
+    // whether a sequence of one row, or all of one call's, can be few in a full table
+    const size_t least = kv->batch > 1 ? 1 : rows;
+    split = AttWork::few(static_cast<uint32_t>(least), static_cast<int>(room));
+    tile = !split || rows > kAttFewRows;
+  }
   cudaError_t e = cudaSuccess;
   if (tile) e = launch_attention_tile(p, view, split);
   if (split && e == cudaSuccess) e = launch_attention_split(p, view, tile);
