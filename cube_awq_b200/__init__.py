@@ -1,7 +1,8 @@
 """cube_awq_b200 — B200 (sm_100a) implementation of the AWQ INT4 hot path of
 joshuawm/cube-awq: the fused dequant-GEMM (decode and prefill kernels) and the
 standalone dequantize kernel, behind the reference's module API; and the
-operators between the linears of a decoder layer (``layer_ops``).
+operators between the linears of a decoder layer (``layer_ops``), put together
+in :class:`AWQDecoderLayer`.
 
     from cube_awq_b200 import AWQGEMMLinearConfig
     layer = AWQGEMMLinearConfig(4096, 4096, 128).with_bias(False).build("cuda:0", torch.float16)
@@ -26,6 +27,7 @@ from .layer_ops import (attention_decode, attention_prefill, rms_norm, rms_norm_
                         rope_table)
 from .modules import (AWQGateUpSiluMul, AWQGEMMLinear, AWQGEMMLinearConfig, AWQLinear,
                       AWQLinearConfig, AWQQKVLinear)
+from .decoder import AWQDecoderLayer
 from .tp import ColumnParallelAWQLinear, RowParallelAWQLinear, TPComm, TPPeers
 from .loader import fuse_decoder_layers, load_awq_linears
 
@@ -40,6 +42,7 @@ if _os.path.exists(_lib.LIB_PATH):
         pass
 
 __all__ = [
+    "AWQDecoderLayer",
     "AWQGateUpSiluMul", "AWQGEMMLinear", "AWQGEMMLinearConfig", "AWQLinear", "AWQLinearConfig",
     "AWQQKVLinear",
     "ColumnParallelAWQLinear", "RowParallelAWQLinear", "TPComm", "TPPeers", "load_awq_linears",
