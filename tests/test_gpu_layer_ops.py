@@ -405,3 +405,65 @@ def test_both_host_paths(cuda_device, compiled, monkeypatch):
     assert out.shape == q.shape and torch.equal(c.v[int(c.table[1, 0]), :, 0], v[3])
     with pytest.raises(CubeAwqError):
         cawq.attention_decode(q[:2], c.k, c.v, c.table, c.lens, window=-1)
+
+
+def test_prefill_many_sequences(cuda_device):
+    # more sequences than the kernels have threads; runs of empty ones
+    seqs = [((i * 7) % 4, (i * 7) % 4 + (i % 5) * 30) if i % 3 else (0, 0) for i in range(1500)]
+    _attend(cuda_device, BF16, seqs, 4, 1, 64, 16, seed=3)
+
+
+def test_decode_many_sequences(cuda_device):
+    _attend(cuda_device, F16, [(1, (i * 37) % 90) for i in range(1000)], 4, 1, 64, 16, seed=4,
+            decode=True)
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (2000, 7)])
+def test_prefill_batches_of_long_and_short_and_prompts(cuda_device, window, sinks):
+    # single tokens and short runs behind long caches (split) beside prompts (tiles)
+    seqs = [(1, 9000), (300, 300), (3, 4001), (16, 7000), (1, 1), (0, 50), (1, 1024), (1, 1023),
+            (100, 5000), (2, 0)]
+    _attend(cuda_device, BF16, seqs, 8, 1, 128, 16, window, sinks, seed=5)
+    _attend(cuda_device, F16, seqs, 14, 2, 64, 24, window, sinks, seed=6, layout="token",
+            evict=bool(window))
+
+
+@pytest.mark.parametrize("new,total", [(1, 3000), (5, 2500), (18, 6000), (19, 800), (40, 9000)])
+def test_prefill_of_one_sequence_with_few_rows(cuda_device, new, total):
+    _attend(cuda_device, F16, [(new, total)], 7, 1, 128, 16, seed=new)
+
+
+@pytest.mark.parametrize("decode", [True, False])
+def test_attention_pages_between_whole_heads(cuda_device, decode):
+    # a page stride that is no whole number of head strides
+    seqs = [(1, 300), (1, 20)] if decode else [(70, 300), (33, 40)]
+    c = Cache(seqs, 3, 128, 16, F16, cuda_device)
+    sh, sp = 16 * 128, 3 * 16 * 128 + 8
+    pool = torch.full((2, c.pages * sp), float("nan"), dtype=F16, device=cuda_device)
+    k, v = (pool[i].as_strided((c.pages, 3, 16, 128), (sp, sh, 128, 1), i * c.pages * sp)
+            for i in range(2))
+    k.copy_(c.k)
+    v.copy_(c.v)
+    q = _randn((c.starts[-1], 12, 128), F16, cuda_device, 2)
+    args = (q, k, v, c.table, c.lens)
+    out = cawq.attention_decode(*args) if decode else cawq.attention_prefill(*args, c.q_start)
+    ref, tol = attention_ref(q, c)
+    assert_within(out, ref, tol)
+
+
+@pytest.mark.parametrize("batch,hq,hkv,length", [(1, 1, 1, 1000), (1, 8, 8, 65), (3, 48, 3, 300),
+                                                 (20, 8, 2, 500), (40, 32, 8, 100), (1, 6, 2, 4096),
+                                                 (2, 64, 64, 129)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_decode_few_row_tiles(cuda_device, batch, hq, hkv, length, d):
+    # calls small enough for a cluster per row tile, of every size, with row
+    # tiles that have fewer keys than the cluster has CTAs
+    lens = [max(0, length - 17 * i * i) for i in range(batch)]
+    _attend(cuda_device, BF16, [(1, t) for t in lens], hq, hkv, d, 16, decode=True, seed=length)
+
+
+def test_attention_scales(cuda_device):
+    seqs = [(130, 200), (3, 2000)]
+    for scale in (-0.2, 1e-3, 2.0):
+        _attend(cuda_device, F16, seqs, 8, 2, 128, 16, scale=scale, qscale=0.5)
+        _attend(cuda_device, F16, [(1, 700)], 8, 2, 128, 16, scale=scale, qscale=0.5, decode=True)
