@@ -129,6 +129,103 @@ __device__ __forceinline__ uint32_t tile_stage_v(int j, int nb) {
   return j + 1 < nb ? 2 * j + 2 : 2 * nb - 1;
 }
 
+// A CTA's tile: its sequence (0xffffffff: none), which of the sequence's tiles,
+// and what the sequence has.
+struct TilePick {
+  uint32_t seq, tile;
+  int first, count, len;
+};
+
+__device__ __forceinline__ uint32_t tile_count(const AttWork& w, int count, int len) {
+  const uint32_t rows = static_cast<uint32_t>(count) * w.group;
+  return w.shared && AttWork::few(rows, len) ? 0u : (rows + kTileRows - 1) / kTileRows;
+}
+
+// Tile number `index` of up to 32 sequences, longest first: lane b counts the
+// tiles of sequence b whose last row is at key block v or later, and v is found
+// by bisection. (Sequence by sequence, one of 2545 tokens after one of 2900
+// began when the first was nearly done: a batch of 7 prompts 95 us, so 73.)
+__device__ __forceinline__ TilePick pick_tile(const AttWork& w, uint32_t index) {
+  const uint32_t lane = threadIdx.x & 31;
+  TilePick t = {lane, 0, 0, 0, 0};
+  uint32_t n = 0;
+  if (lane < w.kv.batch) {
+    w.kv.rows(lane, w.tokens, &t.first, &t.count);
+    t.len = w.kv.len(lane);
+    n = tile_count(w, t.count, t.len);
+  }
+  const uint32_t total = __reduce_add_sync(0xffffffffu, n);
+  if (index >= total) return {0xffffffffu, 0, 0, 0, 0};
+  uint32_t at = index;  // among the tiles of the chosen block
+  uint32_t later = 0;   // this sequence's tiles past it
+  if (w.kv.batch > 1) {
+    const int64_t rows = static_cast<int64_t>(t.count) * w.group;
+    auto reach = [&](int v) -> uint32_t {  // tiles whose last row's position is >= 128 v
+      if (n == 0) return 0;
+      const int64_t row = (static_cast<int64_t>(v) * kTileKeys - (t.len - t.count)) * w.group;
+      if (row <= 0) return n;
+      return row >= rows ? 0u : n - static_cast<uint32_t>(row / kTileRows);
+    };
+    int lo = 0, hi = static_cast<int>(__reduce_max_sync(0xffffffffu, n ? t.len : 0)) / kTileKeys + 1;
+    while (hi - lo > 1) {  // the largest block that still has `index` tiles before or in it
+      const int mid = (lo + hi) >> 1;
+      if (__reduce_add_sync(0xffffffffu, reach(mid)) > index) lo = mid; else hi = mid;
+    }
+    later = reach(lo + 1);
+    at -= __reduce_add_sync(0xffffffffu, later);
+    n = (lo > 0 ? reach(lo) : n) - later;
+  }
+  uint32_t inc = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= static_cast<uint32_t>(o)) inc += v;
+  }
+  const int from = __ffs(__ballot_sync(0xffffffffu, at < inc)) - 1;
+  const uint32_t tiles = tile_count(w, t.count, t.len);
+  t.tile = tiles - 1 - (later + at - (inc - n));
+  t.seq = from;
+  t.tile = __shfl_sync(0xffffffffu, t.tile, from);
+  t.first = __shfl_sync(0xffffffffu, t.first, from);
+  t.count = __shfl_sync(0xffffffffu, t.count, from);
+  t.len = __shfl_sync(0xffffffffu, t.len, from);
+  return t;
+}
+
+// The same of any number of sequences, sequence by sequence, the last tile of
+// each first. All threads; the result is in *pick after the next barrier.
+__device__ __forceinline__ void pick_tile_of_many(const AttWork& w, uint32_t index, uint32_t* sums,
+                                                  TilePick* pick) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t per = (w.kv.batch + kTileThreads - 1) / kTileThreads;
+  const uint32_t b0 = min(w.kv.batch, tid * per), b1 = min(w.kv.batch, b0 + per);
+  int first = 0, count = 0, len = 0;
+  auto tiles = [&](uint32_t b) {
+    w.kv.rows(b, w.tokens, &first, &count);
+    len = w.kv.len(b);
+    return tile_count(w, count, len);
+  };
+  uint32_t n = 0;
+  for (uint32_t b = b0; b < b1; ++b) n += tiles(b);
+  uint32_t inc = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) sums[warp] = inc;
+  if (tid == 0) pick->seq = 0xffffffffu;
+  __syncthreads();
+  uint32_t at = inc - n;
+  for (int i = 0; i < warp; ++i) at += sums[i];
+  if (index >= at && index < at + n) {
+    uint32_t b = b0, last;
+    for (; index >= at + (last = tiles(b)); ++b) at += last;
+    *pick = {b, last - 1 - (index - at), first, count, len};
+  }
+  __syncthreads();
+}
+
 // Pages as heads: how many head strides a page stride is; 0 where the two do
 // not make one dimension (the split kernel then takes the call).
 inline uint64_t tile_heads_per_page(const PagedView& kv) {
@@ -159,10 +256,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* drain = pv_done + 2;  // [2]: of the issuers
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   __shared__ uint32_t s_bad[8], s_sum[kTileThreads / 32];
-  __shared__ struct {
-    uint32_t seq, tile;
-    int first, count, len;
-  } s_tile;
+  __shared__ TilePick s_tile;
   const AttWork& w = a.w;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -188,52 +282,29 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (warp == 16) tmem_alloc(tmem_slot, kTmemCols);
   pdl_wait();
   pdl_launch_dependents();
-  // ---- which tile: the sequences' tiles in order, a sequence's last tile first
-  // (the later a causal tile, the longer it takes)
+  // ---- which tile: those with the most key blocks first, the kv heads of one
+  // side by side
   const uint32_t index = blockIdx.x / w.kv.n_kv, hk = blockIdx.x - index * w.kv.n_kv;
-  {
-    auto tiles = [&](uint32_t b, int* first, int* count, int* len) -> uint32_t {
-      w.kv.rows(b, w.tokens, first, count);
-      *len = w.kv.len(b);
-      const uint32_t rows = static_cast<uint32_t>(*count) * w.group;
-      return w.shared && AttWork::few(rows, *len) ? 0u : (rows + kTileRows - 1) / kTileRows;
-    };
-    const uint32_t per = (w.kv.batch + kTileThreads - 1) / kTileThreads;
-    const uint32_t b0 = min(w.kv.batch, tid * per), b1 = min(w.kv.batch, b0 + per);
-    int first = 0, count = 0, len = 0;
-    uint32_t n = 0, last = 0;
-    for (uint32_t b = b0; b < b1; ++b) n += last = tiles(b, &first, &count, &len);
-    uint32_t inc = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    if (lane == 31) s_sum[warp] = inc;
-    if (tid == 0) s_tile.seq = 0xffffffffu;
-    tc_fence_before();
-    __syncthreads();
-    uint32_t at = inc - n;
-    for (int i = 0; i < warp; ++i) at += s_sum[i];
-    if (index >= at && index < at + n) {
-      uint32_t b = b1 - 1;  // the usual case: a sequence a thread
-      if (per > 1)
-        for (b = b0; index >= at + (last = tiles(b, &first, &count, &len)); ++b) at += last;
-      s_tile = {b, last - 1 - (index - at), first, count, len};
-    }
-    __syncthreads();
-    tc_fence_after();
+  TilePick t;
+  if (w.kv.batch <= 32) {
+    t = pick_tile(w, index);  // by every warp for itself
+  } else {
+    pick_tile_of_many(w, index, s_sum, &s_tile);
+    t = s_tile;
   }
-  const uint32_t b = s_tile.seq;
-  if (b == 0xffffffffu) {  // the grid is sized for the most tiles there can be
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (t.seq == 0xffffffffu) {  // the grid is sized for the most tiles there can be
     if (warp == 16) tmem_dealloc(*tmem_slot, kTmemCols);
     return;
   }
 
   // ---- the tile's rows and key blocks
-  const int first = s_tile.first, count = s_tile.count, len = s_tile.len;
+  const uint32_t b = t.seq;
+  const int first = t.first, count = t.count, len = t.len;
   const uint32_t rows = static_cast<uint32_t>(count) * w.group;
-  const uint32_t p0 = s_tile.tile * kTileRows;
+  const uint32_t p0 = t.tile * kTileRows;
   const bool two = p0 + 128 < rows;
   const int shift = len - count;  // position of the first new token
   const int pos_lo = shift + static_cast<int>(w.by_group.div(p0));
