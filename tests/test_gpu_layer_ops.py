@@ -27,7 +27,8 @@ def _randn(shape, dtype, dev, seed, scale=1.0):
 
 # ----------------------------------------------------------------- RMS norm
 NORM_SIZES = [(1, 4096), (1, 1), (3, 7), (5, 129), (17, 3584), (4, 8200), (2, 16385), (300, 64),
-              (1, 40000)]
+              (1, 40000), (2, 8191), (300, 8192), (2, 16383), (3, 16384), (2, 32768), (300, 1000),
+              (301, 20000), (2, 12000)]
 
 
 def _check_norm(x, w, eps, r, y, h):
