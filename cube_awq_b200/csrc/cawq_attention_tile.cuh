@@ -3,8 +3,13 @@
 //
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c (q . k_j) - m),  c = scale log2(e)
 //
-// over the visible positions j of the row. Bound by the tensor cores: 4 D
-// operations per (row, visible key).
+// over the visible positions j of the row.
+//
+// Bound by the tensor cores: 4 D operations per (row, visible key). Measured,
+// D = 128: 8192 tokens, 32 / 8 heads, f16, 469 us = 1170 TFLOP/s in bursts, 540
+// us = 1020 TFLOP/s sustained, where the GPU's power cap (1000 W) holds the
+// clock at 1.5 GHz; a chunk of 2048 tokens under a window of 4096, 64 / 8 heads,
+// bf16, 285-318 us; 7 ragged prompts, 28 / 4 heads, bf16, 73-78 us.
 //
 // A CTA takes 256 query rows of one (sequence, kv head), as two halves of 128:
 // the rows are the G = n_q / n_kv query heads of consecutive tokens, token by
@@ -15,7 +20,10 @@
 //             cycles, most of them latency; the tensor cores need 1024)
 //   16, 17    tensor memory; one thread each issues the score products and the
 //             second products (one for both spent its waits and commits one
-//             after the other while the tensor cores idled)
+//             after the other while the tensor cores idled). The whole warp
+//             runs the loop and only the instruction is one thread's, which
+//             keeps descriptors in uniform registers: otherwise an MMA took
+//             126 cycles to issue, twice what it takes to run
 //   18, 19    K_j and V_j of block j through one ring of 128-key stages (TMA,
 //             128-byte swizzle; a box is a page's keys, or a power of two of
 //             them that divides the page)
@@ -29,6 +37,12 @@
 // S_h(j + 1) had to wait for PV_h(j), and a block took the softmax and two
 // products.)
 //
+// One CTA per tile: a grid of one CTA per SM whose roles ran on from tile to
+// tile was slower (8192 tokens 530 against 495 us, ragged prompts 150 against
+// 101 us on one box), as were two threads a row that trade their maxima, and
+// exponentials on the FMA pipe for part of the weights (the loop waits for
+// hand-overs and instruction slots, not for the special-function unit).
+//
 // The running maximum m moves only when a row's block maximum exceeds it by
 // more than 2^8: p stays below 2^8 either way, nothing overflows (the sums are
 // fp32, f16 holds 65504), and the row's O is rescaled a few times per row
@@ -38,8 +52,9 @@
 // window) are not read: their boxes are requested outside the tensor and
 // arrive as zeros. The last page's rows past the end may hold anything; for K
 // they only reach masked scores, for V the box is written row by row with
-// zeros past the end, since 0 * NaN is NaN. A page number outside the cache
-// hides its keys (s_bad) and sets the error bit.
+// zeros past the end, since 0 * NaN is NaN. What is loaded for some rows and
+// masked for others has weight 0 there and must be finite. A page number
+// outside the cache hides its keys (s_bad) and sets the error bit.
 //
 // Every wait is bounded (2 s); on a timeout the kernel sets bit 0 of the
 // device error word, stops issuing, waits (bounded) for what it issued, frees

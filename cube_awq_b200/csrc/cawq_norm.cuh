@@ -12,7 +12,7 @@
 // longer ones a CTA. Few rows are latency: one vector a thread (the row's
 // loads all go out at once); many rows are bandwidth: four a thread, so that
 // an SM holds more rows at a time (4099 x 8192 bf16 to e4m3 with the residual:
-// 40.6 us, 5.8 TB/s; 1 x 4096 f16 2.1 us). Rows off 16-byte alignment go
+// 41 us, 5.7 TB/s; 1 x 4096 f16 2.2 us). Rows off 16-byte alignment go
 // element by element, still in registers up to 16384 elements, and longer ones
 // through the caches again in each pass.
 #pragma once

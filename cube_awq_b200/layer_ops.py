@@ -311,7 +311,9 @@ def attention_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     cache that holds them already (cawq_attention_prefill): q [tokens, n_q,
     head_dim] -> the same shape. Rows q_start[b] .. q_start[b + 1] - 1 are the
     last tokens of sequence b; rows of no sequence are left as they are.
-    ``scale``, ``window`` and ``sinks`` as in :func:`attention_decode`."""
+    ``scale``, ``window`` and ``sinks`` as in :func:`attention_decode`. Pages
+    that no new token sees and slots past a sequence's length may hold
+    anything; its other values must be finite."""
     if q_start is None:
         raise ShapeError("attention_prefill needs q_start", _SHAPE)
     return _attention(q, k_cache, v_cache, block_table, seq_lens, q_start, scale, window, sinks,

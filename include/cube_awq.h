@@ -5,7 +5,9 @@
  *   - the fused INT4 dequant-GEMM  Y[M,N] = X[M,K] · ((Q - Z) · S)[K,N]
  *     (reference: src/kernel/awq_kernel_gemm.rs `gemm_awq` / `gemm_awq_decode`),
  *   - the standalone dequantize kernel
- *     (reference: src/kernel/awq_kernel.rs `dequantize_awq_symmetric`).
+ *     (reference: src/kernel/awq_kernel.rs `dequantize_awq_symmetric`),
+ *   - the operators between the linears of a decoder layer: RMS norm, rotary
+ *     append to a paged cache, attention over it (no reference counterpart).
  *
  * Tensor format (AutoAWQ, exactly as the reference reads it):
  *   qweight u32 [K, N/8], qzeros u32 [K/g, N/8], scales F [K/g, N], bias F [N].
@@ -417,8 +419,12 @@ cawq_status cawq_rope_append(const void* q, const void* k, const void* v, const 
  * memory, 16-byte aligned, that no other call uses while this one runs.
  *
  * cawq_attention_decode: one token per sequence (tokens = kv->batch, q_start
- * unused). cawq_attention_prefill: any number per sequence (q_start required);
- * rows of `out` that belong to no sequence are left as they are.
+ * unused); nothing but the visible positions is read. cawq_attention_prefill:
+ * any number per sequence (q_start required); rows of `out` that belong to no
+ * sequence are left as they are. Pages that no new token of a sequence sees and
+ * slots past its length may hold anything; the sequence's other values must be
+ * finite (a weight of 0 times an infinity or NaN is NaN, also for a token that
+ * does not see that position).
  */
 size_t cawq_attention_workspace(const cawq_paged_kv* kv, size_t tokens, size_t n_q);
 
