@@ -20,7 +20,9 @@
 // the lengths are read on the device. A CTA's share may begin or end inside a
 // row tile's keys: it then leaves its part (m, sum, outputs, fp32) in the
 // workspace and a second small kernel joins the parts in order (no atomics:
-// the same bits every time).
+// the same bits every time). Where the keys of each row tile are few, by the
+// table's width, the dealing out costs more than it evens out, and a cluster of
+// CTAs or a single warp takes the row tile instead (att_cluster, att_each).
 //
 // A CTA is four warps that never wait for one another inside a row tile: warp
 // w takes keys 16 w .. 16 w + 15 of each 64-key tile and streams them through
@@ -50,8 +52,9 @@ constexpr uint32_t kAttRowCost = 2;
 // query rows (of a kv head) than the first number, no fewer keys than the
 // second and than the third times its rows.
 constexpr uint32_t kAttFewRows = 128, kAttFewKeys = 1024, kAttFewPerRow = 40;
-constexpr uint32_t kAttCluster = 16;     // most CTAs of a cluster that shares a row tile
+constexpr uint32_t kAttMaxCluster = 16;  // most CTAs of a cluster that shares a row tile
 constexpr uint32_t kAttClusterTiles = 8;  // most key tiles a CTA of it may get
+constexpr uint32_t kAttEachKeys = 256;  // most keys of a row tile that one warp takes
 constexpr int kAttMaxCtas = 320;  // most CTAs of a launch (two per SM)
 
 template <int D>
@@ -236,16 +239,19 @@ __device__ __forceinline__ float* att_slot(char* ws, uint32_t slot) {
 
 // MULTI: sequences may have several new tokens, so rows of a tile see
 // different keys. Without it every visible key is every row's.
-// CLUSTER (one token per sequence): no dealing out; a cluster of CTAs per row
-// tile splits its keys evenly and joins through distributed shared memory, in
-// one launch without a workspace.
-template <int DT, int D, int NT, bool MULTI, bool CLUSTER>
+// kAttCluster (one token per sequence): no dealing out; a cluster of CTAs per
+// row tile splits its keys evenly and joins through distributed shared memory,
+// in one launch without a workspace. kAttEach (the same): a warp per row tile,
+// 16 keys at a time, the row tiles in turn; nothing to join at all.
+enum AttMode { kAttDealt, kAttCluster, kAttEach };
+template <int DT, int D, int NT, bool MULTI, AttMode MODE>
 __global__ void __launch_bounds__(32 * kAttWarps, 2)
     attention_split_kernel(const char* q, char* out, const AttWork w, int64_t ld_q, int64_t ld_o,
                            float scale_log2, char* ws) {
   using T = typename DType<DT>::T;
   using L = AttLayout<D>;
   constexpr int NR = 8 * NT, KS = D / 16;
+  constexpr bool CLUSTER = MODE == kAttCluster, EACH = MODE == kAttEach;
   extern __shared__ __align__(128) uint8_t smem[];
   AttScan& sc = *reinterpret_cast<AttScan*>(smem + L::kRing);  // read before the first merge
   __shared__ float s_m[kAttWarps][NR], s_f[kAttWarps][NR], s_top[NR];
@@ -261,16 +267,31 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
   struct Cursor {
     uint32_t b, hr, tile;
     AttWork::Seq s;
+    uint32_t item;  // EACH: the row tile, of all
   };
   Cursor in;
+  // keys of a unit, and where the warp's own begin; EACH counts units of 16
+  constexpr int UK = EACH ? 16 : kAttKeys;
+  const int own_key = EACH ? 0 : 16 * warp;
+  const uint32_t per_seq = w.kv.n_kv * ((w.group + NR - 1) / NR);  // row tiles, one token each
+  auto place = [&](Cursor& c) {
+    c.b = c.item / per_seq;
+    c.hr = c.item - c.b * per_seq;
+    c.tile = 0;
+    c.s = w.seq(c.b);
+    c.s.tiles = max(1, (c.s.keys + UK - 1) / UK);
+  };
   uint32_t cluster = 1, rank = 0;
-  if constexpr (CLUSTER) {
+  if constexpr (EACH) {
+    in.item = blockIdx.x * kAttWarps + warp;
+    if (in.item >= w.kv.batch * per_seq) return;
+    place(in);
+    left = 1;
+  } else if constexpr (CLUSTER) {
     cluster = cluster_nctarank();
     rank = cluster_ctarank();
-    const uint32_t i = blockIdx.x / cluster;  // the row tile
-    in.b = i / (w.kv.n_kv * ((w.group + NR - 1) / NR));
-    in.s = w.seq(in.b);
-    in.hr = i - in.b * (w.kv.n_kv * ((w.group + NR - 1) / NR));
+    in.item = blockIdx.x / cluster;
+    place(in);
     in.tile = in.s.tiles * rank / cluster;
     left = in.s.tiles * (rank + 1) / cluster - in.tile;
   } else {
@@ -306,6 +327,13 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
   };
   // one tile on, while there are units; false past the CTA's last tile
   auto advance = [&](Cursor& c, int64_t& units) -> bool {
+    if constexpr (EACH) {
+      if (++c.tile < c.s.tiles) return true;
+      c.item += gridDim.x * kAttWarps;
+      if (c.item >= w.kv.batch * per_seq) return false;
+      place(c);
+      return true;
+    }
     --units;
     if (++c.tile < c.s.tiles) return units > 0;
     units -= kAttRowCost;
@@ -315,7 +343,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
   };
   // the lane's position (16 per warp) in the cache: byte offset, -1 if none
   auto lookup = [&](const Cursor& c) -> int64_t {
-    const int i = static_cast<int>(c.tile * kAttKeys) + 16 * warp + (lane & 15);
+    const int i = static_cast<int>(c.tile * UK) + own_key + (lane & 15);
     if (i >= c.s.keys) return -1;
     return w.kv.offset(c.b, c.hr / c.s.row_tiles, static_cast<uint32_t>(c.s.key(i)));
   };
@@ -451,7 +479,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
       for (int c = 0; c < 4; ++c) {
         bool see = c < 2 ? in0 : in1;
         if constexpr (MULTI) {
-          const int key = at.s.key(static_cast<int>(at.tile * kAttKeys) + 16 * warp + g + (c < 2 ? 0 : 8));
+          const int key = at.s.key(static_cast<int>(at.tile * UK) + own_key + g + (c < 2 ? 0 : 8));
           const int p = prow[x][c & 1];
           see = see && key <= p && (w.window == 0 || key > p - w.window || key < w.sinks);
         }
@@ -500,78 +528,111 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
     // ---- the row tile's keys in this CTA end here: join the four warps
     const bool whole = !CLUSTER && tile0 == 0 && done.tile + 1 == done.s.tiles;
     if (go_on) load_rows(at);  // of the next one, while this one ends
+    if constexpr (EACH) {
+      const uint32_t hk = done.hr / done.s.row_tiles;
+      const uint32_t r0 = (done.hr - hk * done.s.row_tiles) * NR;
+      float* own = reinterpret_cast<float*>(smem + L::kRing) + warp * 8 * L::kPad;
 #pragma unroll
-    for (int x = 0; x < NT; ++x)
+      for (int x = 0; x < NT; ++x) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < 2; ++c) {
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], d);
-        if (g == 0) s_m[warp][8 * x + 2 * t4 + c] = m[x][c];
-      }
-    __syncthreads();
-    float* merge = reinterpret_cast<float*>(smem + L::kRing);
-    const uint32_t hk = done.hr / done.s.row_tiles;
-    const uint32_t r0 = (done.hr - hk * done.s.row_tiles) * NR;
-    const int rows = min(NR, static_cast<int>(done.s.count * w.group - r0));
-    // (the rings are done with when the CTA's last row tile ends)
-    float* part = CLUSTER ? reinterpret_cast<float*>(smem)
-                          : att_slot<D, NR>(ws, 2 * blockIdx.x + (first_rows ? 0 : 1));
-    if (!CLUSTER && !go_on && tile0 == 0 && !whole && threadIdx.x == 0) {
-      // the last key tile's unit is this many on from the CTA's end
-      const uint64_t e = u1 - 1 + (done.s.tiles - 1 - done.tile);
-      uint32_t c1 = static_cast<uint32_t>(e * ctas / total);
-      while (att_first_unit(total, c1 + 1, ctas) <= e) ++c1;
-      *note = {c1 - blockIdx.x + 1, first_rows ? 0u : 1u, done.s.first, hk, r0, rows, {0, 0}};
-    }
+          for (int d = 4; d < 32; d <<= 1) l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], d);
+          const float inv = l[x][c] != 0.f ? 1.f / l[x][c] : 0.f;
+          float* dst = own + (2 * t4 + c) * L::kPad;
 #pragma unroll
-    for (int x = 0; x < NT; ++x) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int r = 8 * x + 2 * t4 + c;
-        float top = s_m[0][r];
-#pragma unroll
-        for (int i = 1; i < kAttWarps; ++i) top = fmaxf(top, s_m[i][r]);
-        const float f = exp2_approx(m[x][c] - (top == -INFINITY ? 0.f : top));
-        if (g == 0) {  // this warp's sum on the common scale
-          s_f[warp][r] = l[x][c] * f;
-          if (warp == 0) s_top[r] = top;
-        }
-        float* dst = merge + (warp * 8 + 2 * t4 + c) * L::kPad;
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          dst[16 * i + g] = o[x][i][c] * f;
-          dst[16 * i + g + 8] = o[x][i][c + 2] * f;
-        }
-      }
-      __syncthreads();
-      for (int e = threadIdx.x; e < 8 * D; e += 32 * kAttWarps) {
-        const int r = 8 * x + e / D, c = e % D;
-        if (r >= rows) break;
-        float sum = 0.f, v = 0.f;
-#pragma unroll
-        for (int i = 0; i < kAttWarps; ++i) {
-          sum += s_f[i][r];
-          v += merge[(i * 8 + e / D) * L::kPad + c];
-        }
-        if (whole) {
-          const uint32_t tok = w.by_group.div(r0 + r);
-          T* dst = reinterpret_cast<T*>(out + (done.s.first + tok) * ld_o +
-                                        static_cast<int64_t>(hk * w.group + r0 + r - tok * w.group) * (2 * D));
-          dst[c] = DType<DT>::from_f32(sum != 0.f ? v / sum : 0.f);
-        } else {
-          part[2 * NR + r * D + c] = v;
-          if (c == 0) {
-            part[r] = s_top[r];
-            part[NR + r] = sum;
+          for (int i = 0; i < KS; ++i) {
+            dst[16 * i + g] = o[x][i][c] * inv;
+            dst[16 * i + g + 8] = o[x][i][c + 2] * inv;
           }
         }
+        __syncwarp();
+        const int rows = min(8, static_cast<int>(w.group - r0) - 8 * x);  // one token
+        for (int e = 2 * lane; e < rows * D; e += 64) {
+          const int r = e / D, c = e % D;
+          const float* v = own + r * L::kPad + c;
+          *reinterpret_cast<uint32_t*>(out + done.s.first * ld_o +
+                                       static_cast<int64_t>(hk * w.group + r0 + 8 * x + r) * (2 * D) +
+                                       2 * c) = pack2<DT>(v[0], v[1]);
+        }
+        __syncwarp();
       }
+      if (!go_on) break;
+      clear();
+    } else {
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], d);
+          if (g == 0) s_m[warp][8 * x + 2 * t4 + c] = m[x][c];
+        }
       __syncthreads();
+      float* merge = reinterpret_cast<float*>(smem + L::kRing);
+      const uint32_t hk = done.hr / done.s.row_tiles;
+      const uint32_t r0 = (done.hr - hk * done.s.row_tiles) * NR;
+      const int rows = min(NR, static_cast<int>(done.s.count * w.group - r0));
+      // (the rings are done with when the CTA's last row tile ends)
+      float* part = CLUSTER ? reinterpret_cast<float*>(smem)
+                            : att_slot<D, NR>(ws, 2 * blockIdx.x + (first_rows ? 0 : 1));
+      if (!CLUSTER && !go_on && tile0 == 0 && !whole && threadIdx.x == 0) {
+        // the last key tile's unit is this many on from the CTA's end
+        const uint64_t e = u1 - 1 + (done.s.tiles - 1 - done.tile);
+        uint32_t c1 = static_cast<uint32_t>(e * ctas / total);
+        while (att_first_unit(total, c1 + 1, ctas) <= e) ++c1;
+        *note = {c1 - blockIdx.x + 1, first_rows ? 0u : 1u, done.s.first, hk, r0, rows, {0, 0}};
+      }
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int r = 8 * x + 2 * t4 + c;
+          float top = s_m[0][r];
+#pragma unroll
+          for (int i = 1; i < kAttWarps; ++i) top = fmaxf(top, s_m[i][r]);
+          const float f = exp2_approx(m[x][c] - (top == -INFINITY ? 0.f : top));
+          if (g == 0) {  // this warp's sum on the common scale
+            s_f[warp][r] = l[x][c] * f;
+            if (warp == 0) s_top[r] = top;
+          }
+          float* dst = merge + (warp * 8 + 2 * t4 + c) * L::kPad;
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            dst[16 * i + g] = o[x][i][c] * f;
+            dst[16 * i + g + 8] = o[x][i][c + 2] * f;
+          }
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < 8 * D; e += 32 * kAttWarps) {
+          const int r = 8 * x + e / D, c = e % D;
+          if (r >= rows) break;
+          float sum = 0.f, v = 0.f;
+#pragma unroll
+          for (int i = 0; i < kAttWarps; ++i) {
+            sum += s_f[i][r];
+            v += merge[(i * 8 + e / D) * L::kPad + c];
+          }
+          if (whole) {
+            const uint32_t tok = w.by_group.div(r0 + r);
+            T* dst = reinterpret_cast<T*>(out + (done.s.first + tok) * ld_o +
+                                          static_cast<int64_t>(hk * w.group + r0 + r - tok * w.group) * (2 * D));
+            dst[c] = DType<DT>::from_f32(sum != 0.f ? v / sum : 0.f);
+          } else {
+            part[2 * NR + r * D + c] = v;
+            if (c == 0) {
+              part[r] = s_top[r];
+              part[NR + r] = sum;
+            }
+          }
+        }
+        __syncthreads();
+      }
+      if (!go_on) break;
+      first_rows = false;
+      tile0 = 0;
+      clear();
     }
-    if (!go_on) break;
-    first_rows = false;
-    tile0 = 0;
-    clear();
   }
   cp_async_wait<0>();
   if constexpr (CLUSTER) {
@@ -584,22 +645,22 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
     const uint32_t hk = at.hr / at.s.row_tiles, r0 = (at.hr - hk * at.s.row_tiles) * NR;
     const int rows = min(NR, static_cast<int>(at.s.count * w.group - r0));
     const uint32_t base = smem_u32(own);
+    // the parts' maxima and sums here first, then their outputs
+    float* ml = own + NR * (D + 2);  // [cluster][2 NR]
+    for (uint32_t e = threadIdx.x; e < cluster * 2 * NR; e += 32 * kAttWarps)
+      ml[e] = ld_shared_cluster_f32(map_shared_rank(base + 4 * (e % (2 * NR)), e / (2 * NR)));
+    __syncthreads();
+#pragma unroll 4
     for (int e = threadIdx.x + 32 * kAttWarps * rank; e < rows * D; e += 32 * kAttWarps * cluster) {
       const int r = e / D, c = e % D;
-      float m_[kAttCluster], top = -INFINITY, sum = 0.f, v = 0.f;
-#pragma unroll
-      for (uint32_t i = 0; i < kAttCluster; ++i)
-        m_[i] = i < cluster ? ld_shared_cluster_f32(map_shared_rank(base + 4 * r, i)) : -INFINITY;
-#pragma unroll
-      for (uint32_t i = 0; i < kAttCluster; ++i) top = fmaxf(top, m_[i]);
+      float top = -INFINITY, sum = 0.f, v = 0.f;
+      for (uint32_t i = 0; i < cluster; ++i) top = fmaxf(top, ml[2 * NR * i + r]);
       const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-      for (uint32_t i = 0; i < kAttCluster; ++i) {
-        if (i >= cluster) break;
-        const float k = exp2_approx(m_[i] - ref);
-        const uint32_t p = map_shared_rank(base, i);
-        sum += ld_shared_cluster_f32(p + 4 * (NR + r)) * k;
-        v += ld_shared_cluster_f32(p + 4 * (2 * NR + e)) * k;
+#pragma unroll 4
+      for (uint32_t i = 0; i < cluster; ++i) {
+        const float k = exp2_approx(ml[2 * NR * i + r] - ref);
+        sum += ml[2 * NR * i + NR + r] * k;
+        v += ld_shared_cluster_f32(map_shared_rank(base + 4 * (2 * NR + e), i)) * k;
       }
       const uint32_t tok = w.by_group.div(r0 + r);
       T* dst = reinterpret_cast<T*>(out + (at.s.first + tok) * ld_o +
@@ -699,27 +760,45 @@ inline uint64_t att_most_units(size_t batch, size_t tokens, size_t group, size_t
   return tiles * row_tiles * n_kv;
 }
 
-// CTAs of a cluster for calls whose row tiles are few and whose keys, by what
-// the table (or the window) holds, make no more than kAttClusterTiles key tiles
-// for each of its CTAs; 0 for the others. One launch that joins in shared
-// memory against two: 1 sequence of 1000 tokens, 32 heads, f16, 7.1 against 9.6 us.
-// Long or ragged batches need the dealt-out units.
-inline uint32_t att_cluster(const AttentionProblem& p, const PagedView& kv, uint32_t nr) {
-  if (kv.q_start) return 0;
-  const uint64_t group = p.n_q / kv.n_kv, row_tiles = kv.batch * kv.n_kv * ((group + nr - 1) / nr);
-  uint64_t keys = static_cast<uint64_t>(kv.width) * kv.page.d;
-  if (p.window > 0) keys = std::min<uint64_t>(keys, static_cast<uint64_t>(p.window) + p.sinks);
-  const uint64_t tiles = (keys + kAttKeys - 1) / kAttKeys;
-  uint32_t c = kAttCluster;
-  while (c > 1 && (row_tiles * c > 2ull * p.sm_count || c >= 2 * tiles)) c /= 2;
-  return row_tiles * c <= 2ull * p.sm_count && tiles <= c * kAttClusterTiles ? c : 0;
+// What the host knows of a call with one token per sequence: its row tiles, and
+// the most keys that one can have by the table (or the window).
+struct AttBounds {
+  uint64_t row_tiles, keys;
+};
+inline AttBounds att_bounds(const AttentionProblem& p, const PagedView& kv, uint32_t nr) {
+  const uint64_t group = p.n_q / kv.n_kv;
+  AttBounds b = {static_cast<uint64_t>(kv.batch) * kv.n_kv * ((group + nr - 1) / nr),
+                 static_cast<uint64_t>(kv.width) * kv.page.d};
+  if (p.window > 0) b.keys = std::min<uint64_t>(b.keys, static_cast<uint64_t>(p.window) + p.sinks);
+  return b;
+}
+
+// CTAs of a cluster for calls whose row tiles are few and have no more than
+// kAttClusterTiles key tiles for each of its CTAs; 0 for the others. One launch
+// that joins in shared memory against two: 1 sequence of 1000 tokens, 32 heads,
+// f16, 7.1 against 9.6 us. Long or ragged batches need the dealt-out units.
+inline uint32_t att_cluster(const AttBounds& b, int sm_count) {
+  const uint64_t tiles = (b.keys + kAttKeys - 1) / kAttKeys;
+  uint32_t c = kAttMaxCluster;
+  while (c > 1 && (b.row_tiles * c > 2ull * sm_count || c >= 2 * tiles)) c /= 2;
+  return c > 1 && tiles <= c * kAttClusterTiles ? c : 0;
+}
+
+// Otherwise a warp per row tile where no row tile has many keys: no parts, no
+// joins. us a call against the dealt-out units (bf16, D = 128, 32 / 8 heads):
+// 256 sequences of 16 / 128 / 250 tokens 7.4 / 25.6 / 44.8 against
+// 21.2 / 37.2 / 53.7; 32 sequences 3.6 / 8.6 / 14.8 against 5.6 / 11.9 / 14.7.
+// Above the limit the longest sequence's one warp is what the call waits for:
+// 256 sequences of 1 to 1000 tokens 63.4 against 42.1.
+inline bool att_each(const AttBounds& b) {
+  return b.keys <= kAttEachKeys && b.row_tiles < (1ull << 30);
 }
 
 template <int DT, int D, int NT>
 cudaError_t launch_attention_cluster_t(const AttentionProblem& p, const PagedView& kv,
                                        uint32_t cluster) {
   static uint64_t done = 0;
-  auto kern = attention_split_kernel<DT, D, NT, false, true>;
+  auto kern = attention_split_kernel<DT, D, NT, false, kAttCluster>;
   if (!(p.device < 64 && (done >> p.device & 1))) {
     const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
                                                cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -738,11 +817,29 @@ cudaError_t launch_attention_cluster_t(const AttentionProblem& p, const PagedVie
                     cluster);
 }
 
+template <int DT, int D, int NT>
+cudaError_t launch_attention_each_t(const AttentionProblem& p, const PagedView& kv) {
+  static uint64_t done = 0;
+  auto kern = attention_split_kernel<DT, D, NT, false, kAttEach>;
+  const cudaError_t e = allow_smem(kern, AttLayout<D>::kSmem, p.device, &done);
+  if (e != cudaSuccess) return e;
+  AttWork w = att_work(p, kv, 8 * NT, false);
+  const char* q = static_cast<const char*>(p.q);
+  char *out = static_cast<char*>(p.out), *ws = nullptr;
+  int64_t ld_q = static_cast<int64_t>(p.ld_q) * 2, ld_o = static_cast<int64_t>(p.ld_out) * 2;
+  float sl = p.scale * kLog2e;
+  void* a[] = {&q, &out, &w, &ld_q, &ld_o, &sl, &ws};
+  const uint64_t items = static_cast<uint64_t>(kv.batch) * kv.n_kv * ((w.group + 8 * NT - 1) / (8 * NT));
+  const uint32_t ctas = static_cast<uint32_t>(
+      std::min<uint64_t>((items + kAttWarps - 1) / kAttWarps, 2 * p.sm_count));
+  return launch_pdl(kern, dim3(ctas), 32 * kAttWarps, AttLayout<D>::kSmem, p.stream, a);
+}
+
 template <int DT, int D, int NT, bool MULTI>
 cudaError_t launch_attention_split_t(const AttentionProblem& p, const PagedView& kv,
                                      bool shared) {
   static uint64_t done = 0;  // a lost update only repeats the call
-  auto kern = attention_split_kernel<DT, D, NT, MULTI, false>;
+  auto kern = attention_split_kernel<DT, D, NT, MULTI, kAttDealt>;
   cudaError_t e = allow_smem(kern, AttLayout<D>::kSmem, p.device, &done);
   if (e != cudaSuccess) return e;
   AttWork w = att_work(p, kv, 8 * NT, shared);
@@ -778,10 +875,14 @@ cudaError_t launch_attention_split(const AttentionProblem& p, const PagedView& k
                                    bool shared) {
   const bool multi = kv.q_start != nullptr;
   const bool two = att_row_tile(p.n_q / kv.n_kv, multi) == 16;
-  const uint32_t cluster = att_cluster(p, kv, two ? 16 : 8);
-#define CAWQ_ATT(DT, D)                                                    \
-  (cluster ? two ? launch_attention_cluster_t<DT, D, 2>(p, kv, cluster)    \
-                 : launch_attention_cluster_t<DT, D, 1>(p, kv, cluster)    \
+  const AttBounds bounds = att_bounds(p, kv, two ? 16 : 8);
+  const uint32_t cluster = multi ? 0 : att_cluster(bounds, p.sm_count);
+  const bool each = !multi && cluster == 0 && att_each(bounds);
+#define CAWQ_ATT(DT, D)                                                              \
+  (each ? two ? launch_attention_each_t<DT, D, 2>(p, kv)                             \
+              : launch_attention_each_t<DT, D, 1>(p, kv)                             \
+   : cluster ? two ? launch_attention_cluster_t<DT, D, 2>(p, kv, cluster)            \
+                   : launch_attention_cluster_t<DT, D, 1>(p, kv, cluster)            \
    : multi ? launch_attention_split_t<DT, D, 2, true>(p, kv, shared)                 \
          : two ? launch_attention_split_t<DT, D, 2, false>(p, kv, shared)          \
                : launch_attention_split_t<DT, D, 1, false>(p, kv, shared))

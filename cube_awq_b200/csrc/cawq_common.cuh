@@ -209,20 +209,6 @@ __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t count) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
 }
 
-// The same barrier; true for all if the predicate is for one.
-__device__ __forceinline__ bool named_bar_or(uint32_t id, bool v, uint32_t count = 64) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %3, 0;\n\t"
-      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(id), "r"(count), "r"(static_cast<uint32_t>(v))
-      : "memory");
-  return r != 0;
-}
-
 // Address of output element (row, col): columns [0, c1) live in p0 (row
 // stride ld0), [c1, c2) in p1 and [c2, n) in p2 (the q / k / v outputs of a
 // fused qkv projection); a single output has c1 = c2 = 0xFFFFFFFF. Fields,

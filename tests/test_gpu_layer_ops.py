@@ -463,6 +463,25 @@ def test_decode_few_row_tiles(cuda_device, batch, hq, hkv, length, d):
     _attend(cuda_device, BF16, [(1, t) for t in lens], hq, hkv, d, 16, decode=True, seed=length)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("batch,hq,hkv,d", [(400, 8, 8, 64), (300, 64, 4, 128), (70, 5, 5, 128),
+                                            (257, 9, 3, 64), (150, 24, 2, 128)])
+@pytest.mark.parametrize("page,longest", [(16, 256), (8, 256), (24, 250), (16, 17), (64, 64), (16, 257)])
+def test_decode_many_short_sequences(cuda_device, dtype, batch, hq, hkv, d, page, longest):
+    # tables short enough for a warp per row tile, more of them than warps; and
+    # one page past that
+    lens = [longest if i == 7 else (i * i * 13 + 5 * i) % (longest + 1) for i in range(batch)]
+    _attend(cuda_device, dtype, [(1, t) for t in lens], hq, hkv, d, page, decode=True, seed=batch)
+
+
+@pytest.mark.parametrize("layout", ["head", "token", "pair"])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (17, 0), (200, 56), (250, 7)])
+def test_decode_many_sequences_in_short_windows(cuda_device, layout, window, sinks):
+    lens = [(i * 131) % 1500 for i in range(160)]
+    _attend(cuda_device, BF16, [(1, t) for t in lens], 16, 8, 128, 16, decode=True, evict=True,
+            window=window, sinks=sinks, layout=layout)
+
+
 def test_attention_scales(cuda_device):
     seqs = [(130, 200), (3, 2000)]
     for scale in (-0.2, 1e-3, 2.0):
