@@ -54,7 +54,8 @@ constexpr uint32_t kAttRowCost = 2;
 constexpr uint32_t kAttFewRows = 128, kAttFewKeys = 1024, kAttFewPerRow = 40;
 constexpr uint32_t kAttMaxCluster = 16;  // most CTAs of a cluster that shares a row tile
 constexpr uint32_t kAttClusterTiles = 8;  // most key tiles a CTA of it may get
-constexpr uint32_t kAttEachKeys = 256;  // most keys of a row tile that one warp takes
+// Most keys of a row tile that one warp takes: of those in two waves of CTAs, of others.
+constexpr uint32_t kAttEachFew = 128, kAttEachKeys = 256;
 constexpr int kAttMaxCtas = 320;  // most CTAs of a launch (two per SM)
 
 template <int D>
@@ -254,7 +255,12 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
   constexpr bool CLUSTER = MODE == kAttCluster, EACH = MODE == kAttEach;
   extern __shared__ __align__(128) uint8_t smem[];
   AttScan& sc = *reinterpret_cast<AttScan*>(smem + L::kRing);  // read before the first merge
-  __shared__ float s_m[kAttWarps][NR], s_f[kAttWarps][NR], s_top[NR];
+  // The warps' maxima and sums for their join stand in the merge rows' padding:
+  // with 640 bytes more a CTA, two would not fit on an SM at D = 128 (250
+  // sequences of 1000 tokens, 16 / 1 heads, dealt out: 63 against 45 us).
+  float* merge = reinterpret_cast<float*>(smem + L::kRing);
+  auto s_m = [&](int i, int r) -> float& { return merge[(8 * i + (r & 7)) * L::kPad + D + (r >> 3)]; };
+  auto s_f = [&](int i, int r) -> float& { return merge[(8 * i + (r & 7)) * L::kPad + D + 2 + (r >> 3)]; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
 
@@ -311,6 +317,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
     const uint32_t r = static_cast<uint32_t>(rel - static_cast<uint64_t>(in.hr) * (in.s.tiles + kAttRowCost));
     in.tile = r < kAttRowCost ? 0 : r - kAttRowCost;
     left -= r < kAttRowCost ? kAttRowCost - r : 0;
+    __syncthreads();  // sc is read: the merge rows may be written
     if (left <= 0) return;  // nothing but the cost of a row tile that the next CTA begins
   }
   Cursor at = in;
@@ -526,7 +533,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
     const bool go_on = advance(at, todo);
     if (go_on && at.tile != 0) continue;
     // ---- the row tile's keys in this CTA end here: join the four warps
-    const bool whole = !CLUSTER && tile0 == 0 && done.tile + 1 == done.s.tiles;
+    const bool whole = CLUSTER ? cluster == 1 : tile0 == 0 && done.tile + 1 == done.s.tiles;
     if (go_on) load_rows(at);  // of the next one, while this one ends
     if constexpr (EACH) {
       const uint32_t hk = done.hr / done.s.row_tiles;
@@ -566,10 +573,9 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], d);
-          if (g == 0) s_m[warp][8 * x + 2 * t4 + c] = m[x][c];
+          if (g == 0) s_m(warp, 8 * x + 2 * t4 + c) = m[x][c];
         }
       __syncthreads();
-      float* merge = reinterpret_cast<float*>(smem + L::kRing);
       const uint32_t hk = done.hr / done.s.row_tiles;
       const uint32_t r0 = (done.hr - hk * done.s.row_tiles) * NR;
       const int rows = min(NR, static_cast<int>(done.s.count * w.group - r0));
@@ -588,14 +594,11 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int r = 8 * x + 2 * t4 + c;
-          float top = s_m[0][r];
+          float top = s_m(0, r);
 #pragma unroll
-          for (int i = 1; i < kAttWarps; ++i) top = fmaxf(top, s_m[i][r]);
+          for (int i = 1; i < kAttWarps; ++i) top = fmaxf(top, s_m(i, r));
           const float f = exp2_approx(m[x][c] - (top == -INFINITY ? 0.f : top));
-          if (g == 0) {  // this warp's sum on the common scale
-            s_f[warp][r] = l[x][c] * f;
-            if (warp == 0) s_top[r] = top;
-          }
+          if (g == 0) s_f(warp, r) = l[x][c] * f;  // this warp's sum on the common scale
           float* dst = merge + (warp * 8 + 2 * t4 + c) * L::kPad;
 #pragma unroll
           for (int i = 0; i < KS; ++i) {
@@ -604,24 +607,30 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
           }
         }
         __syncthreads();
-        for (int e = threadIdx.x; e < 8 * D; e += 32 * kAttWarps) {
+        for (int e = 2 * threadIdx.x; e < 8 * D; e += 64 * kAttWarps) {
           const int r = 8 * x + e / D, c = e % D;
           if (r >= rows) break;
-          float sum = 0.f, v = 0.f;
+          float sum = 0.f, v0 = 0.f, v1 = 0.f;
 #pragma unroll
           for (int i = 0; i < kAttWarps; ++i) {
-            sum += s_f[i][r];
-            v += merge[(i * 8 + e / D) * L::kPad + c];
+            sum += s_f(i, r);
+            const float2 v = *reinterpret_cast<const float2*>(merge + (i * 8 + e / D) * L::kPad + c);
+            v0 += v.x;
+            v1 += v.y;
           }
           if (whole) {
-            const uint32_t tok = w.by_group.div(r0 + r);
-            T* dst = reinterpret_cast<T*>(out + (done.s.first + tok) * ld_o +
-                                          static_cast<int64_t>(hk * w.group + r0 + r - tok * w.group) * (2 * D));
-            dst[c] = DType<DT>::from_f32(sum != 0.f ? v / sum : 0.f);
+            const uint32_t tok = MULTI ? w.by_group.div(r0 + r) : 0;
+            const float inv = sum != 0.f ? 1.f / sum : 0.f;
+            *reinterpret_cast<uint32_t*>(out + (done.s.first + tok) * ld_o +
+                                         static_cast<int64_t>(hk * w.group + r0 + r - tok * w.group) * (2 * D) +
+                                         2 * c) = pack2<DT>(v0 * inv, v1 * inv);
           } else {
-            part[2 * NR + r * D + c] = v;
+            *reinterpret_cast<float2*>(part + 2 * NR + r * D + c) = make_float2(v0, v1);
             if (c == 0) {
-              part[r] = s_top[r];
+              float top = s_m(0, r);
+#pragma unroll
+              for (int i = 1; i < kAttWarps; ++i) top = fmaxf(top, s_m(i, r));
+              part[r] = top;
               part[NR + r] = sum;
             }
           }
@@ -636,6 +645,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
   }
   cp_async_wait<0>();
   if constexpr (CLUSTER) {
+    if (cluster == 1) return;
     // every CTA of the cluster joins its share of the row tile's elements
     float* own = reinterpret_cast<float*>(smem);
     if (left0 <= 0) {  // more CTAs than key tiles
@@ -651,21 +661,22 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
       ml[e] = ld_shared_cluster_f32(map_shared_rank(base + 4 * (e % (2 * NR)), e / (2 * NR)));
     __syncthreads();
 #pragma unroll 4
-    for (int e = threadIdx.x + 32 * kAttWarps * rank; e < rows * D; e += 32 * kAttWarps * cluster) {
+    for (int e = 2 * (threadIdx.x + 32 * kAttWarps * rank); e < rows * D; e += 64 * kAttWarps * cluster) {
       const int r = e / D, c = e % D;
-      float top = -INFINITY, sum = 0.f, v = 0.f;
+      float top = -INFINITY, sum = 0.f, v0 = 0.f, v1 = 0.f;
       for (uint32_t i = 0; i < cluster; ++i) top = fmaxf(top, ml[2 * NR * i + r]);
       const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll 4
       for (uint32_t i = 0; i < cluster; ++i) {
         const float k = exp2_approx(ml[2 * NR * i + r] - ref);
+        const uint32_t src = map_shared_rank(base + 4 * (2 * NR + e), i);
         sum += ml[2 * NR * i + NR + r] * k;
-        v += ld_shared_cluster_f32(map_shared_rank(base + 4 * (2 * NR + e), i)) * k;
+        v0 += ld_shared_cluster_f32(src) * k;
+        v1 += ld_shared_cluster_f32(src + 4) * k;
       }
-      const uint32_t tok = w.by_group.div(r0 + r);
-      T* dst = reinterpret_cast<T*>(out + (at.s.first + tok) * ld_o +
-                                    static_cast<int64_t>(hk * w.group + r0 + r - tok * w.group) * (2 * D));
-      dst[c] = DType<DT>::from_f32(sum != 0.f ? v / sum : 0.f);
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;
+      *reinterpret_cast<uint32_t*>(out + at.s.first * ld_o + static_cast<int64_t>(hk * w.group + r0 + r) * (2 * D) +
+                                   2 * c) = pack2<DT>(v0 * inv, v1 * inv);
     }
     cluster_sync_all();  // no CTA leaves while another reads its part
   }
@@ -773,23 +784,31 @@ inline AttBounds att_bounds(const AttentionProblem& p, const PagedView& kv, uint
   return b;
 }
 
-// CTAs of a cluster for calls whose row tiles are few and have no more than
-// kAttClusterTiles key tiles for each of its CTAs; 0 for the others. One launch
-// that joins in shared memory against two: 1 sequence of 1000 tokens, 32 heads,
-// f16, 7.1 against 9.6 us. Long or ragged batches need the dealt-out units.
+// CTAs of a cluster per row tile, for calls that need no more than two waves of
+// them and give none more than kAttClusterTiles key tiles; 0 for the others. One
+// launch that joins in shared memory, or has nothing to join, against two: 1
+// sequence of 1000 tokens, 32 heads, f16, 6.8 against 9.5 us (c = 8); 250
+// sequences of 500 tokens, 16 / 1 heads, 17.5 against 33.6, of 1 to 500 tokens
+// 12.4 against 18.6 (c = 1). Long or ragged batches need the dealt-out units:
+// 32 sequences of 1 to 1000 tokens, 32 / 8 heads, 17.0 against 13.9.
+// Several CTAs pay from four key tiles on (1 sequence of 128 tokens: 4.2 us with
+// one, 4.9 with two; of 250: 5.7 and, with four, 5.1).
 inline uint32_t att_cluster(const AttBounds& b, int sm_count) {
-  const uint64_t tiles = (b.keys + kAttKeys - 1) / kAttKeys;
+  const uint64_t tiles = (b.keys + kAttKeys - 1) / kAttKeys, wave = 2ull * sm_count;
   uint32_t c = kAttMaxCluster;
-  while (c > 1 && (b.row_tiles * c > 2ull * sm_count || c >= 2 * tiles)) c /= 2;
-  return c > 1 && tiles <= c * kAttClusterTiles ? c : 0;
+  while (c > 1 && (b.row_tiles * c > wave || c >= 2 * tiles || tiles < 4)) c /= 2;
+  if (tiles > c * kAttClusterTiles || b.row_tiles > 2 * wave) return 0;
+  return b.row_tiles <= wave || b.keys > kAttEachFew ? c : 0;
 }
 
-// Otherwise a warp per row tile where no row tile has many keys: no parts, no
-// joins. us a call against the dealt-out units (bf16, D = 128, 32 / 8 heads):
-// 256 sequences of 16 / 128 / 250 tokens 7.4 / 25.6 / 44.8 against
-// 21.2 / 37.2 / 53.7; 32 sequences 3.6 / 8.6 / 14.8 against 5.6 / 11.9 / 14.7.
-// Above the limit the longest sequence's one warp is what the call waits for:
-// 256 sequences of 1 to 1000 tokens 63.4 against 42.1.
+// Otherwise a warp per row tile where no row tile has many keys: no joins at
+// all. us a call against the dealt-out units (bf16, D = 128, 32 / 8 heads): 256
+// sequences of 16 / 128 / 250 tokens 7.3 / 25.9 / 44.4 against 19.2 / 35.4 /
+// 52.9. Above kAttEachKeys the longest sequence's one warp is what the call
+// waits for: 256 sequences of 1 to 1000 tokens 63.9 against 41.2. The same
+// holds above kAttEachFew where the row tiles leave half the warps idle: 64
+// sequences of 1 to 250 tokens 14.6 against 9.4 with a CTA for each, of 64
+// tokens 5.8 against 7.2.
 inline bool att_each(const AttBounds& b) {
   return b.keys <= kAttEachKeys && b.row_tiles < (1ull << 30);
 }

@@ -474,6 +474,14 @@ def test_decode_many_short_sequences(cuda_device, dtype, batch, hq, hkv, d, page
     _attend(cuda_device, dtype, [(1, t) for t in lens], hq, hkv, d, page, decode=True, seed=batch)
 
 
+@pytest.mark.parametrize("batch,hq,hkv", [(296, 3, 1), (297, 16, 1), (64, 32, 8), (37, 56, 8), (148, 20, 4)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("longest", [128, 129, 190, 512, 513])
+def test_decode_one_or_two_row_tiles_for_each_cta(cuda_device, batch, hq, hkv, d, longest):
+    lens = [longest if i == 3 else (i * i * 7 + 11 * i) % (longest + 1) for i in range(batch)]
+    _attend(cuda_device, BF16, [(1, t) for t in lens], hq, hkv, d, 16, decode=True, seed=longest)
+
+
 @pytest.mark.parametrize("layout", ["head", "token", "pair"])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (17, 0), (200, 56), (250, 7)])
 def test_decode_many_sequences_in_short_windows(cuda_device, layout, window, sinks):
