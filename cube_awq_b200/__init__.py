@@ -10,7 +10,7 @@ in :class:`AWQDecoderLayer`.
     y = layer.forward(x)          # x [..., 4096] -> y [..., 4096]
 
 All compute runs in the CUDA library ``libcube_awq.so`` (C ABI:
-``include/cube_awq.h``); importing this package loads it, and without it
+``include/cube_awq.h``), loaded by the first call that needs it; without it
 every compute call raises ImportError (there is no CPU fallback). Build it
 with ``python -m cube_awq_b200.build``.
 """
@@ -31,15 +31,10 @@ from .decoder import AWQDecoderLayer
 from .tp import ColumnParallelAWQLinear, RowParallelAWQLinear, TPComm, TPPeers
 from .loader import fuse_decoder_layers, load_awq_linears
 
-import os as _os
-
-if _os.path.exists(_lib.LIB_PATH):
-    try:
-        _lib.lib()  # load now; without the library every compute call raises (no CPU fallback)
-    except (OSError, AttributeError):
-        # a library from an older build: `python -m cube_awq_b200.build` must
-        # still be able to run; every compute call raises until it is rebuilt
-        pass
+# libcube_awq.so is loaded by the first call that needs it (which raises if it
+# has not been built), not here: a process that imports the package and then
+# rebuilds a stale library would run two copies, the one loaded before and the
+# one that the compiled host path loads, with a device error word each.
 
 __all__ = [
     "AWQDecoderLayer",

@@ -227,14 +227,5 @@ def lib():
     return _lib
 
 
-def forget() -> None:
-    """Drops the loaded library, so that the next call loads the file that is
-    there now: after a rebuild the compiled host path would load it, and the two
-    copies would have an error word each."""
-    global _lib
-    with _lock:
-        _lib = None
-
-
 def last_error() -> str:
     return lib().cawq_last_error().decode("utf-8", "replace")

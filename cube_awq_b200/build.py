@@ -105,8 +105,6 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB_PATH)
-    from . import _lib
-    _lib.forget()  # importing the package loaded the one before
     return LIB_PATH
 
 

@@ -1,33 +1,19 @@
-"""A rebuild in a process that has loaded the library: the next call loads the
-new file, the one that the compiled host path would load too."""
+"""Importing the package does not load the library: a process that imports it
+and then rebuilds the library runs the new one, and only that."""
 
-import os
-import shutil
+import subprocess
+import sys
 
-from cube_awq_b200 import _lib, build
+CODE = """
+import cube_awq_b200, cube_awq_b200.build
+from cube_awq_b200 import _lib
+maps = lambda: "libcube_awq.so" in open("/proc/self/maps").read()
+assert not maps()
+cube_awq_b200.version()
+assert maps()
+"""
 
 
-def test_a_rebuilt_library_is_loaded_anew(tmp_path, monkeypatch):
-    path = str(tmp_path / "libcube_awq.so")
-    shutil.copy(_lib.LIB_PATH, path)
-    for module in (_lib, build):
-        monkeypatch.setattr(module, "LIB_PATH", path)
-    monkeypatch.setattr(_lib, "_lib", None)
-    before = _lib.lib()
-    assert _lib.lib() is before
-
-    class Done:
-        returncode = 0
-
-    def link(cmd, **_):
-        shutil.copy(before._name, cmd[cmd.index("-o") + 1])
-        return Done()
-
-    monkeypatch.setattr(build, "_compile", lambda src, verbose, extra: src)
-    monkeypatch.setattr(build.subprocess, "run", link)
-    inode = os.stat(path).st_ino
-    assert build.build(force=True) == path
-    assert os.stat(path).st_ino != inode
-    after = _lib.lib()
-    assert after is not before and after._handle != before._handle
-    assert after.cawq_version() == before.cawq_version()
+def test_the_library_is_loaded_by_the_first_call_not_by_the_import():
+    r = subprocess.run([sys.executable, "-c", CODE], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
