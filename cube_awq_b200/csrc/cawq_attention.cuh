@@ -48,10 +48,9 @@ constexpr int kAttStages = 3;
 // long ones left the CTAs with the short ones last (64 sequences of 1 to 8000
 // tokens, 28 / 4 heads: 62 us).
 constexpr uint32_t kAttRowCost = 2;
-// A sequence is for the split kernel rather than the tile kernel with no more
-// query rows (of a kv head) than the first number, no fewer keys than the
-// second and than the third times its rows.
-constexpr uint32_t kAttFewRows = 128, kAttFewKeys = 1024, kAttFewPerRow = 40;
+// A sequence of at most so many query rows (of a kv head) is for the split
+// kernel where a call's keys are worth splitting (AttLoad).
+constexpr uint32_t kAttFewRows = 128;
 constexpr uint32_t kAttMaxCluster = 16;  // most CTAs of a cluster that shares a row tile
 constexpr uint32_t kAttClusterTiles = 8;  // most key tiles a CTA of it may get
 // Most keys of a row tile that one warp takes: of those in two waves of CTAs, of others.
@@ -114,17 +113,7 @@ struct AttWork {
   uint32_t tokens, group, row_tile;  // group = n_q / n_kv, row_tile = NR
   FastDiv by_group;
   int window, sinks;
-  bool shared;  // the tile kernel takes the sequences whose rows are not few
-
-  // Few rows are bound by their keys' bytes and gain from the split; many, or
-  // few keys, do as well in a tile. Per call, us split / tiles (D = 128, bf16,
-  // one sequence): 16 rows, 8 kv heads at 500 / 3000 / 20000 keys 11 / 23 / 41
-  // against 11 / 34 / 186; 64 rows 22 / 31 / 101 against 11 / 35 / 187; 128
-  // rows 25 / 45 / 181 against 12 / 35 / 188.
-  __host__ __device__ __forceinline__ static bool few(uint32_t rows, int len) {
-    const uint32_t n = static_cast<uint32_t>(len);
-    return rows <= kAttFewRows && n >= kAttFewKeys && n >= kAttFewPerRow * rows;
-  }
+  bool shared;  // both kernels run: the tile kernel takes what the split kernel leaves
 
   // Sequence b: its rows, its keys in order of position without the hidden
   // ones between the sinks and the window of its first new token, and its
@@ -144,13 +133,71 @@ struct AttWork {
     s.head = min(sinks, s.start);
     s.keys = s.len - s.start + s.head;
     s.row_tiles = (static_cast<uint32_t>(s.count) * group + row_tile - 1) / row_tile;
-    s.tiles = s.count > 0 && (!shared || few(s.count * group, s.len))
+    s.tiles = s.count > 0 && (!shared || s.count * group <= kAttFewRows)
                   ? max(1, (s.keys + kAttKeys - 1) / kAttKeys)
                   : 0u;
     return s;
   }
   __device__ __forceinline__ uint64_t units(const Seq& s) const {
     return s.tiles ? static_cast<uint64_t>(s.tiles + kAttRowCost) * s.row_tiles * kv.n_kv : 0;
+  }
+};
+
+// Whether a call's sequences of few rows go to the split kernel, by what all its
+// sequences need. A tile reads a key in 9.4 ns and the GPU streams 11.8 keys a
+// ns, kPole in that time; the split kernel reads a sequence's keys once per row
+// tile of 16, but no CTA waits for the longest. So it gains where the longest
+// sequence of few rows, less what its two launches cost, has more keys than all
+// row tiles together have per kPole. us split / tiles (bf16, D = 128, 8 kv heads,
+// all of 1000 / 4000 / 16000 tokens): 1 sequence of 16 rows 15 / 17 / 27 against
+// 15 / 43 / 150, of 128 rows 20 / 35 / 93 against 16 / 44 / 152; 8 of 16 rows
+// 20 / 39 / 99 against 16 / 46 / 155, of 64 rows 44 / 108 / 351 against
+// 17 / 46 / 156; 32 of 16 rows and 1 to 8000 tokens 33 against 81.
+struct AttLoad {
+  static constexpr uint32_t kPole = 111, kLaunch = 850;
+  uint64_t keys;     // of the row tiles, or tiles, of all sequences
+  uint32_t longest;  // of few rows
+  __host__ __device__ __forceinline__ bool splits() const {
+    return longest > kLaunch && static_cast<uint64_t>(longest - kLaunch) * kPole > keys;
+  }
+  // one sequence
+  __device__ __forceinline__ static AttLoad of(const AttWork& w, int count, int len) {
+    AttLoad a = {0, 0};
+    if (count <= 0 || len <= 0) return a;
+    const int64_t rows = static_cast<int64_t>(count) * w.group;
+    int64_t n = len;
+    if (w.window > 0) n = min(n, static_cast<int64_t>(w.window) + w.sinks + count);
+    const bool few = rows <= kAttFewRows;
+    if (few) a.longest = static_cast<uint32_t>(n);
+    a.keys = static_cast<uint64_t>(n) * w.kv.n_kv * ((rows + (few ? 15 : 255)) / (few ? 16 : 256));
+    return a;
+  }
+  __device__ __forceinline__ void add(const AttLoad& o) {
+    keys += o.keys;
+    longest = max(longest, o.longest);
+  }
+  __device__ __forceinline__ AttLoad of_warp() const {
+    AttLoad a = *this;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      a.add({__shfl_xor_sync(0xffffffffu, a.keys, o), __shfl_xor_sync(0xffffffffu, a.longest, o)});
+    return a;
+  }
+  // all sequences, by all of a CTA's warps; `part` holds one per warp
+  template <int WARPS>
+  __device__ __forceinline__ static AttLoad of_call(const AttWork& w, AttLoad* part) {
+    AttLoad a = {0, 0};
+    for (uint32_t b = threadIdx.x; b < w.kv.batch; b += 32 * WARPS) {
+      int first, count;
+      w.kv.rows(b, w.tokens, &first, &count);
+      a.add(of(w, count, w.kv.len(b)));
+    }
+    a = a.of_warp();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
+    __syncthreads();
+    a = part[0];
+    for (int i = 1; i < WARPS; ++i) a.add(part[i]);
+    return a;
   }
 };
 
@@ -163,6 +210,7 @@ struct AttScan {
   uint64_t sums[W];       // of the warps
   uint64_t total, before;
   uint32_t seq;
+  AttLoad loads[W];
 };
 
 __device__ __forceinline__ void att_scan(const AttWork& w, AttScan& sc) {
@@ -301,6 +349,10 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
     in.tile = in.s.tiles * rank / cluster;
     left = in.s.tiles * (rank + 1) / cluster - in.tile;
   } else {
+    if (w.shared) {
+      if (threadIdx.x == 0) note->parts = 0;
+      if (!AttLoad::of_call<kAttWarps>(w, sc.loads).splits()) return;
+    }
     att_scan(w, sc);
     total = sc.total;
     ctas = att_ctas(total, gridDim.x);

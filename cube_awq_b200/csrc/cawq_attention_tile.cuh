@@ -151,9 +151,10 @@ struct TilePick {
   int first, count, len;
 };
 
-__device__ __forceinline__ uint32_t tile_count(const AttWork& w, int count, int len) {
+// few: the split kernel takes the sequences of few rows
+__device__ __forceinline__ uint32_t tile_count(const AttWork& w, int count, bool few) {
   const uint32_t rows = static_cast<uint32_t>(count) * w.group;
-  return w.shared && AttWork::few(rows, len) ? 0u : (rows + kTileRows - 1) / kTileRows;
+  return few && rows <= kAttFewRows ? 0u : (rows + kTileRows - 1) / kTileRows;
 }
 
 // Tile number `index` of up to 32 sequences, longest first: lane b counts the
@@ -163,12 +164,13 @@ __device__ __forceinline__ uint32_t tile_count(const AttWork& w, int count, int 
 __device__ __forceinline__ TilePick pick_tile(const AttWork& w, uint32_t index) {
   const uint32_t lane = threadIdx.x & 31;
   TilePick t = {lane, 0, 0, 0, 0};
-  uint32_t n = 0;
   if (lane < w.kv.batch) {
     w.kv.rows(lane, w.tokens, &t.first, &t.count);
     t.len = w.kv.len(lane);
-    n = tile_count(w, t.count, t.len);
   }
+  const bool few = w.shared && AttLoad::of(w, t.count, t.len).of_warp().splits();
+  const uint32_t tiles = tile_count(w, t.count, few);
+  uint32_t n = tiles;
   const uint32_t total = __reduce_add_sync(0xffffffffu, n);
   if (index >= total) return {0xffffffffu, 0, 0, 0, 0};
   uint32_t at = index;  // among the tiles of the chosen block
@@ -197,7 +199,6 @@ __device__ __forceinline__ TilePick pick_tile(const AttWork& w, uint32_t index) 
     if (lane >= static_cast<uint32_t>(o)) inc += v;
   }
   const int from = __ffs(__ballot_sync(0xffffffffu, at < inc)) - 1;
-  const uint32_t tiles = tile_count(w, t.count, t.len);
   t.tile = tiles - 1 - (later + at - (inc - n));
   t.seq = from;
   t.tile = __shfl_sync(0xffffffffu, t.tile, from);
@@ -210,7 +211,8 @@ __device__ __forceinline__ TilePick pick_tile(const AttWork& w, uint32_t index) 
 // The same of any number of sequences, sequence by sequence, the last tile of
 // each first. All threads; the result is in *pick after the next barrier.
 __device__ __forceinline__ void pick_tile_of_many(const AttWork& w, uint32_t index, uint32_t* sums,
-                                                  TilePick* pick) {
+                                                  AttLoad* loads, TilePick* pick) {
+  const bool few = w.shared && AttLoad::of_call<kTileThreads / 32>(w, loads).splits();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t per = (w.kv.batch + kTileThreads - 1) / kTileThreads;
   const uint32_t b0 = min(w.kv.batch, tid * per), b1 = min(w.kv.batch, b0 + per);
@@ -218,7 +220,7 @@ __device__ __forceinline__ void pick_tile_of_many(const AttWork& w, uint32_t ind
   auto tiles = [&](uint32_t b) {
     w.kv.rows(b, w.tokens, &first, &count);
     len = w.kv.len(b);
-    return tile_count(w, count, len);
+    return tile_count(w, count, few);
   };
   uint32_t n = 0;
   for (uint32_t b = b0; b < b1; ++b) n += tiles(b);
@@ -304,7 +306,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (w.kv.batch <= 32) {
     t = pick_tile(w, index);  // by every warp for itself
   } else {
-    pick_tile_of_many(w, index, s_sum, &s_tile);
+    pick_tile_of_many(w, index, s_sum, reinterpret_cast<AttLoad*>(smem), &s_tile);
     t = s_tile;
   }
   tc_fence_before();

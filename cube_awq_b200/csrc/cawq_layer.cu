@@ -204,21 +204,22 @@ static cawq_status attention(const void* q, void* out, const cawq_paged_kv* kv, 
                               static_cast<int>(std::min(sinks, kMaxInt)), dtype, workspace,
                               dev.sm_count, dev.device, static_cast<cudaStream_t>(stream)};
   const PagedView view = paged_view(*kv, 2, decode);
-  // Long sequences with few query rows go to the split kernel, the others to
-  // the tile kernel (AttWork::few). The lengths are the device's; the host goes
-  // by what it knows, the rows in all and what the table can hold: one kernel
-  // for one sequence, for few rows in all, for short tables and for batches of
+  // Sequences of few query rows go to the split kernel where splitting their
+  // keys pays, the others to the tile kernel (AttLoad). The lengths are the
+  // device's; the host goes by what it knows, the rows in all and the most keys
+  // that the table or the window allow: one kernel for one sequence, for few
+  // rows in all that pay at that length, for short tables and for batches of
   // prompts (1024 rows a sequence and more); else both, each on its own
-  // sequences (an empty one costs about 10 us: the second of a batch of prompts
-  // took it from 95 to 124 us).
+  // sequences (an empty one costs 5 us).
   const size_t rows = tokens * (n_q / kv->n_kv);  // of a kv head, in all
-  const size_t room = kv->table_width * kv->page_size;
+  size_t keys = kv->table_width * kv->page_size;
+  if (window > 0) keys = std::min(keys, std::min(window, kMaxInt) + std::min(sinks, kMaxInt) + tokens);
   bool split = decode || tile_heads_per_page(view) == 0, tile = !split;
-  if (tile && (rows <= kAttFewRows || (kv->batch > 1 && rows < 1024 * kv->batch))) {
-    // whether a sequence of one row, or all of one call's, can be few in a full table
-    const size_t least = kv->batch > 1 ? 1 : rows;
-    split = AttWork::few(static_cast<uint32_t>(least), static_cast<int>(room));
-    tile = !split || rows > kAttFewRows;
+  if (tile && keys > AttLoad::kLaunch && (kv->batch == 1 ? rows <= kAttFewRows : rows < 1024 * kv->batch)) {
+    const size_t row_tiles = kv->batch == 1 ? (rows + 15) / 16 : rows / 16 + std::min(kv->batch, tokens);
+    const uint32_t longest = static_cast<uint32_t>(std::min(keys, kMaxInt));
+    tile = !(rows <= kAttFewRows && AttLoad{row_tiles * kv->n_kv * longest, longest}.splits());
+    split = kv->batch > 1 || !tile;
   }
   cudaError_t e = cudaSuccess;
   if (tile) e = launch_attention_tile(p, view, split);

@@ -429,6 +429,20 @@ def test_prefill_batches_of_long_and_short_and_prompts(cuda_device, window, sink
             evict=bool(window))
 
 
+@pytest.mark.parametrize("long", [900, 6000])
+@pytest.mark.parametrize("batch", [5, 32, 33, 70])
+@pytest.mark.parametrize("prompt", [0, 33, 600])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1500, 4)])
+def test_prefill_of_many_short_runs_and_a_long_one(cuda_device, long, batch, prompt, window, sinks):
+    # what one sequence has decides which kernel takes the others' rows, empty
+    # sequences and 128 rows (of a kv head) among them, 132 and a prompt left out
+    seqs = [(0, 30) if i % 4 == 3 else (1 + i % 3, 1 + i % 3 + (i * i * 29) % 300) for i in range(batch)]
+    seqs[1], seqs[2], seqs[batch - 1] = (32, 700), (33, 700), (3, long)
+    if prompt:
+        seqs[4] = (prompt, prompt + 11)
+    _attend(cuda_device, BF16, seqs, 8, 2, 64, 16, window=window, sinks=sinks, seed=batch + long)
+
+
 @pytest.mark.parametrize("new,total", [(1, 3000), (5, 2500), (18, 6000), (19, 800), (40, 9000)])
 def test_prefill_of_one_sequence_with_few_rows(cuda_device, new, total):
     _attend(cuda_device, F16, [(new, total)], 7, 1, 128, 16, seed=new)
