@@ -6,12 +6,13 @@
 // over the visible positions j of the row.
 //
 // Bound by the tensor cores: 4 D operations per (row, visible key). Measured,
-// D = 128: 8192 tokens, 32 / 8 heads, f16, 469 us = 1170 TFLOP/s in bursts, 540
-// us = 1020 TFLOP/s sustained, where the GPU's power cap (1000 W) holds the
+// D = 128: 8192 tokens, 32 / 8 heads, f16, 458 us = 1200 TFLOP/s in bursts, 532
+// us = 1030 TFLOP/s sustained, where the GPU's power cap (1000 W) holds the
 // clock at 1.5 GHz; a chunk of 2048 tokens under a window of 4096, 64 / 8 heads,
-// bf16, 285-318 us; 7 ragged prompts, 28 / 4 heads, bf16, 73-78 us.
+// bf16, 280-311 us; 7 ragged prompts, 28 / 4 heads, bf16, 68-84 us.
 //
-// A CTA takes 256 query rows of one (sequence, kv head), as two halves of 128:
+// A CTA takes 256 query rows of one (sequence, kv head), as two halves of 128
+// (one, where that leaves half the SMs idle):
 // the rows are the G = n_q / n_kv query heads of consecutive tokens, token by
 // token, so the heads that share keys share their loads whatever G is, and the
 // key blocks of 128 that the causal mask or the window cut are few. Warps:
@@ -66,7 +67,7 @@
 
 namespace cawq {
 
-constexpr int kTileRows = 256;
+constexpr uint32_t kTileRows = 256;  // or half of them (launch_attention_tile_t)
 constexpr int kTileKeys = 128;
 constexpr int kTileThreads = 640;
 constexpr int kTileLoaders = 2;  // warps that issue the loads of a stage
@@ -154,7 +155,7 @@ struct TilePick {
 // few: the split kernel takes the sequences of few rows
 __device__ __forceinline__ uint32_t tile_count(const AttWork& w, int count, bool few) {
   const uint32_t rows = static_cast<uint32_t>(count) * w.group;
-  return few && rows <= kAttFewRows ? 0u : (rows + kTileRows - 1) / kTileRows;
+  return few && rows <= kAttFewRows ? 0u : (rows + w.row_tile - 1) / w.row_tile;
 }
 
 // Tile number `index` of up to 32 sequences, longest first: lane b counts the
@@ -181,7 +182,7 @@ __device__ __forceinline__ TilePick pick_tile(const AttWork& w, uint32_t index) 
       if (n == 0) return 0;
       const int64_t row = (static_cast<int64_t>(v) * kTileKeys - (t.len - t.count)) * w.group;
       if (row <= 0) return n;
-      return row >= rows ? 0u : n - static_cast<uint32_t>(row / kTileRows);
+      return row >= rows ? 0u : n - static_cast<uint32_t>(row / w.row_tile);
     };
     int lo = 0, hi = static_cast<int>(__reduce_max_sync(0xffffffffu, n ? t.len : 0)) / kTileKeys + 1;
     while (hi - lo > 1) {  // the largest block that still has `index` tiles before or in it
@@ -321,11 +322,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const uint32_t b = t.seq;
   const int first = t.first, count = t.count, len = t.len;
   const uint32_t rows = static_cast<uint32_t>(count) * w.group;
-  const uint32_t p0 = t.tile * kTileRows;
-  const bool two = p0 + 128 < rows;
+  const uint32_t p0 = t.tile * w.row_tile, p1 = min(p0 + w.row_tile, rows);
+  const bool two = p0 + 128 < p1;
   const int shift = len - count;  // position of the first new token
   const int pos_lo = shift + static_cast<int>(w.by_group.div(p0));
-  const int pos_hi = shift + static_cast<int>(w.by_group.div(min(p0 + kTileRows, rows) - 1));
+  const int pos_hi = shift + static_cast<int>(w.by_group.div(p1 - 1));
   const int start = w.window > 0 ? max(0, pos_lo - w.window + 1) : 0;
   const int head = (min(w.sinks, start) + kTileKeys - 1) / kTileKeys;  // blocks that hold sinks
   const int main0 = max(start / kTileKeys, head);
@@ -780,7 +781,15 @@ cudaError_t launch_attention_tile_t(const AttentionProblem& p, const PagedView& 
   CUtensorMap mk, mv;
   if (!encode_cache(&mk, DT, kv.k, kv, D, a.box) || !encode_cache(&mv, DT, kv.v, kv, D, a.box))
     return cudaErrorInvalidValue;
-  const uint64_t tiles = p.tokens * a.w.group / kTileRows + std::min<uint64_t>(kv.batch, p.tokens);
+  // Tiles of one half where the CTAs of two would leave half the SMs idle, since
+  // a block of keys takes less time with one: 77 tokens, 14 / 2 heads, D = 64,
+  // 6.9 against 7.8 us, 500 tokens 10.6 against 13.0; 64 to 500 new tokens after
+  // 2000, 32 / 8 heads, D = 128, 27 to 31.5 against 35 to 40.
+  uint64_t tiles = 0;
+  for (a.w.row_tile = kTileRows;; a.w.row_tile /= 2) {
+    tiles = p.tokens * a.w.group / a.w.row_tile + std::min<uint64_t>(kv.batch, p.tokens);
+    if (a.w.row_tile < kTileRows || 2 * tiles * kv.n_kv > static_cast<uint64_t>(p.sm_count)) break;
+  }
   void* args[] = {&mk, &mv, &a};
   return launch_pdl(kern, dim3(static_cast<uint32_t>(tiles * kv.n_kv)), kTileThreads,
                     TileLayout<D>::kSmem, p.stream, args);
