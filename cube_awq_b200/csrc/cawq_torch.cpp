@@ -204,13 +204,15 @@ bool paged(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
   return true;
 }
 
-// Token stride of a [tokens, heads, d] operand with dense heads.
+// Token stride of a [tokens, heads, d] operand with dense heads; false where
+// tokens share memory (a stride of 0 would mean "dense" to the C call).
 bool heads_of(const at::Tensor& t, const On& on, c10::ScalarType type, int64_t tokens,
               int64_t heads, int64_t d, size_t* ld) {
   if (!on.here(t) || t.scalar_type() != type || t.dim() != 3 || t.size(0) != tokens ||
       t.size(1) != heads || t.size(2) != d)
     return false;
   if (t.numel() > 0 && (t.stride(2) != 1 || (heads > 1 && t.stride(1) != d))) return false;
+  if (tokens > 1 && t.stride(0) < heads * d) return false;
   *ld = static_cast<size_t>(tokens > 1 ? t.stride(0) : heads * d);
   return true;
 }

@@ -56,11 +56,15 @@ def _same_device(*tensors: Optional[torch.Tensor]) -> None:
 
 
 def _rows(name: str, t: torch.Tensor, shape, dtype: torch.dtype) -> None:
-    """A [rows, d] operand: its shape and type, unit column stride."""
+    """A [rows, d] operand: its shape and type, unit column stride, and rows that
+    do not overlap (a broadcast one's stride of 0 means "dense" to the C calls)."""
     if t.dtype != dtype:
         raise DTypeError(f"{name} must be {dtype}, got {t.dtype}", _lib.CAWQ_ERR_DTYPE)
     if tuple(t.shape) != tuple(shape) or (t.numel() > 0 and t.shape[1] > 1 and t.stride(1) != 1):
         raise ShapeError(f"{name} must be {list(shape)} with unit column stride", _SHAPE)
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ShapeError(f"{name}: row stride {t.stride(0)} is below its {t.shape[1]} columns "
+                         "(a broadcast operand has to be made contiguous)", _SHAPE)
 
 
 def _norm(x, weight, eps, residual, out, out_dtype, residual_out, scales):
@@ -124,8 +128,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight over the last
     dimension, computed in fp32 and rounded once each. Without a residual h is
     None (it would be x). x, residual [..., d] f32, f16 or bf16, contiguous or
-    2-D with a unit column stride. ``out`` may be x, ``residual_out`` may be
-    ``residual`` (the residual stream updated in place)."""
+    2-D with a unit column stride and a row stride of at least d (a broadcast
+    operand is refused). ``out`` may be x, ``residual_out`` may be ``residual``
+    (the residual stream updated in place)."""
     ext = _torch_ext()
     if ext is not None:
         r = ext.rms_norm(x, weight, eps, residual, out, residual_out)
@@ -197,7 +202,8 @@ def _paged(k_cache, v_cache, block_table, seq_lens, q_start, dtype) -> _lib.Page
 
 def _heads(name: str, t: torch.Tensor, heads: Optional[int], d: int, dtype: torch.dtype,
            tokens: Optional[int] = None) -> int:
-    """Token stride of a [tokens, heads, head_dim] operand with dense heads."""
+    """Token stride of a [tokens, heads, head_dim] operand with dense heads and
+    tokens that do not overlap (0 means "dense" to the C calls)."""
     if t.dtype != dtype:
         raise DTypeError(f"{name} must be {dtype}, got {t.dtype}", _lib.CAWQ_ERR_DTYPE)
     if t.dim() != 3 or t.shape[2] != d or (heads is not None and t.shape[1] != heads) or \
@@ -206,6 +212,9 @@ def _heads(name: str, t: torch.Tensor, heads: Optional[int], d: int, dtype: torc
         raise ShapeError(f"{name} must be {want}, got {list(t.shape)}", _SHAPE)
     if t.numel() > 0 and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != d)):
         raise ShapeError(f"{name} must hold its heads dense (strides [ld, {d}, 1])", _SHAPE)
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1] * d:
+        raise ShapeError(f"{name}: token stride {t.stride(0)} is below its {t.shape[1]} x {d} elements "
+                         "(a broadcast operand has to be made contiguous)", _SHAPE)
     return t.stride(0) if t.shape[0] > 1 else t.shape[1] * d
 
 
@@ -217,8 +226,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope: torch.T
     to the cache (cawq_rope_append); returns the turned q.
 
     q [tokens, n_q, head_dim], k and v [tokens, n_kv, head_dim] f16 or bf16,
-    heads dense, any token stride (views of a fused projection's output will
-    do); rope fp32 [positions, head_dim] (:func:`rope_table`). Element i of a
+    heads dense, any token stride of at least the heads' width (views of a fused
+    projection's output will do, a broadcast operand is refused); rope fp32 [positions, head_dim] (:func:`rope_table`). Element i of a
     head turns with element i + head_dim / 2. ``out`` may be q itself. Without
     ``q_start`` there is one new token per sequence. A token of an empty slot
     (negative position) gets a zero q and is not stored."""
