@@ -689,6 +689,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                     (rr & 7) * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
         }
         fence_proxy_async_smem();
+        __syncwarp();  // lane 0's arrival speaks for all lanes' writes
       }
       // the boxes are dealt out to the loaders' lanes
       const uint32_t box = lane * kTileLoaders + loader;
