@@ -56,7 +56,9 @@ struct PagedView {
     *count = e - a;
   }
   // the sequence of row t (batch if none): how many q_start[b + 1] are <= t,
-  // by a search that a whole warp makes with 32 probes a step
+  // by a search that a whole warp makes with 32 probes a step. Row t may lie
+  // outside rows(b) all the same: before q_start[0], or where q_start does not
+  // ascend.
   __device__ __forceinline__ uint32_t sequence(uint32_t t) const {
     if (!q_start) return t;
     const uint32_t lane = threadIdx.x & 31;

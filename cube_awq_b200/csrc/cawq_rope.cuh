@@ -53,7 +53,10 @@ __global__ void __launch_bounds__(kRopeThreads)
   if (b < kv.batch) {
     int first, count;
     kv.rows(b, tokens, &first, &count);
-    pos = kv.len(b) - count + static_cast<int>(t) - first;
+    // a row before q_start[0], or one that starts out of order left outside its
+    // sequence, has no place: with it pos < len(b), which offset() relies on
+    if (static_cast<int>(t) >= first && static_cast<int>(t) < first + count)
+      pos = kv.len(b) - count + static_cast<int>(t) - first;
   }
   if (pos >= static_cast<int>(rope_rows)) {
     atomicOr(&g_cawq_device_error, kErrCache);

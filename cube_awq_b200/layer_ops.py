@@ -230,7 +230,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope: torch.T
     projection's output will do, a broadcast operand is refused); rope fp32 [positions, head_dim] (:func:`rope_table`). Element i of a
     head turns with element i + head_dim / 2. ``out`` may be q itself. Without
     ``q_start`` there is one new token per sequence. A token of an empty slot
-    (negative position) gets a zero q and is not stored."""
+    (negative position), or of no sequence (before ``q_start[0]`` or from
+    ``q_start[batch]`` on), gets a zero q and is not stored."""
     ext = _torch_ext()
     if ext is not None:
         r = ext.rope_append(q, k, v, rope, k_cache, v_cache, block_table, seq_lens, q_start, out)

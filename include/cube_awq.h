@@ -398,8 +398,10 @@ typedef struct cawq_paged_kv {
  * [rope_rows, head_dim]: row p holds the head_dim / 2 cosines, then the sines,
  * of position p, and element i turns with element i + head_dim / 2. q_out may
  * be q's own buffer. Rounded once to `dtype` (CAWQ_F16 or CAWQ_BF16). A token
- * with a negative position gets a zero q_out and no place in the cache; one at
- * or past rope_rows the same, with bit 2 of the device error word.
+ * with a negative position gets a zero q_out and no place in the cache, and so
+ * does a row that belongs to no sequence (before q_start[0], or from
+ * q_start[batch] on); one at or past rope_rows the same, with bit 2 of the
+ * device error word.
  */
 cawq_status cawq_rope_append(const void* q, const void* k, const void* v, const float* rope,
                              size_t rope_rows, void* q_out, const cawq_paged_kv* kv,

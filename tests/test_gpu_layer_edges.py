@@ -43,3 +43,51 @@ def test_prefill_of_caches_that_end_inside_a_box(cuda_device, page, d):
     assert_within(out, ref, tol)
     for _ in range(30):
         assert torch.equal(call(), out)
+
+
+def _rope_args(dev, tokens, hq=4, hkv=2, d=64, seed=0):
+    q, k, v = (_randn((tokens, h, d), F16, dev, seed + i) for i, h in enumerate((hq, hkv, hkv)))
+    return q, k, v, cawq.rope_table(200, d, device=dev)
+
+
+def test_rows_outside_all_sequences_are_left_out(cuda_device):
+    # a part of a batch on the tensors of the whole: rows before q_start[0] and
+    # from q_start[batch] on are no sequence's
+    seqs = [(3, 100), (2, 9)]
+    c = Cache(seqs, 2, 64, 16, F16, cuda_device)
+    q_start = c.q_start + 5
+    q, k, v, rope = _rope_args(cuda_device, 13)
+    out = cawq.rope_append(q, k, v, rope, c.k, c.v, c.table, c.lens, q_start=q_start)
+    want = Cache(seqs, 2, 64, 16, F16, cuda_device)
+    mine = slice(5, 10)
+    got = cawq.rope_append(q[mine], k[mine], v[mine], rope, want.k, want.v, want.table, want.lens,
+                           q_start=want.q_start)
+    assert torch.equal(out[mine], got) and not out[:5].any() and not out[10:].any()
+    for a, b in ((c.k, want.k), (c.v, want.v)):
+        assert torch.equal(a.nan_to_num(nan=7.0), b.nan_to_num(nan=7.0))
+    keep = torch.full_like(q, 3.0)
+    att = cawq.attention_prefill(q, c.k, c.v, c.table, c.lens, q_start, out=keep)
+    assert (att[:5] == 3).all() and (att[10:] == 3).all()
+    assert torch.equal(att[mine], cawq.attention_prefill(q[mine], c.k, c.v, c.table, c.lens, c.q_start))
+
+
+def test_row_starts_that_do_not_ascend_stay_inside_the_cache(cuda_device):
+    # such starts break a precondition; what they name is then undefined, but
+    # no token goes past its sequence's length. The table's rows lie in a wider
+    # one, whose other entries name a page that nothing may touch.
+    g = torch.Generator().manual_seed(0)
+    batch, tokens, page = 6, 24, 8
+    starts = [[0, 9, 1, 2, 8, 3, 24]] + [torch.randint(0, tokens + 1, (batch + 1,), generator=g).tolist()
+                                         for _ in range(60)]
+    q, k, v, rope = _rope_args(cuda_device, tokens)
+    for s in starts:
+        kc = torch.zeros((2 * batch + 1, 2, page, 64), dtype=F16, device=cuda_device)
+        vc = kc.clone()
+        wide = torch.full((batch, 8), 2 * batch, dtype=torch.int32, device=cuda_device)
+        wide[:, :2] = torch.arange(2 * batch, device=cuda_device).view(batch, 2)
+        lens = _i32([13, 16, 1, 5, 0, 9], cuda_device)
+        out = cawq.rope_append(q, k, v, rope, kc, vc, wide[:, :2], lens, q_start=_i32(s, cuda_device))
+        assert out.shape == q.shape and not kc[-1].any() and not vc[-1].any()
+        for b, n in enumerate(lens.tolist()):  # nor past a length inside the table
+            flat = kc[2 * b:2 * b + 2].transpose(1, 2).reshape(2 * page, -1)
+            assert not flat[n:].any()
