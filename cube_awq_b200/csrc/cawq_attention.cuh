@@ -124,12 +124,17 @@ struct AttWork {
     uint32_t tiles, row_tiles;
     __device__ __forceinline__ int key(int c) const { return c < head ? c : c - head + start; }
   };
+  // the first position in the window of position pos (which may lie so far
+  // below zero that pos - window passes 32 bits)
+  __device__ __forceinline__ int window_start(int pos) const {
+    return window > 0 && pos >= window ? pos - window + 1 : 0;
+  }
   __device__ __forceinline__ Seq seq(uint32_t b) const {
     Seq s;
     kv.rows(b, tokens, &s.first, &s.count);
     s.len = kv.len(b);
     const int pos = s.len - s.count;  // of the first new token
-    s.start = window > 0 ? max(0, pos - window + 1) : 0;
+    s.start = window_start(pos);
     s.head = min(sinks, s.start);
     s.keys = s.len - s.start + s.head;
     s.row_tiles = (static_cast<uint32_t>(s.count) * group + row_tile - 1) / row_tile;
@@ -540,7 +545,7 @@ __global__ void __launch_bounds__(32 * kAttWarps, 2)
         if constexpr (MULTI) {
           const int key = at.s.key(static_cast<int>(at.tile * UK) + own_key + g + (c < 2 ? 0 : 8));
           const int p = prow[x][c & 1];
-          see = see && key <= p && (w.window == 0 || key > p - w.window || key < w.sinks);
+          see = see && key <= p && (w.window == 0 || p - key < w.window || key < w.sinks);
         }
         v[c] = see ? s[x][c] * scale_log2 : -INFINITY;
       }

@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int shift = len - count;  // position of the first new token
   const int pos_lo = shift + static_cast<int>(w.by_group.div(p0));
   const int pos_hi = shift + static_cast<int>(w.by_group.div(p1 - 1));
-  const int start = w.window > 0 ? max(0, pos_lo - w.window + 1) : 0;
+  const int start = w.window_start(pos_lo);
   const int head = (min(w.sinks, start) + kTileKeys - 1) / kTileKeys;  // blocks that hold sinks
   const int main0 = max(start / kTileKeys, head);
   const int nb = pos_hi < 0 ? 0 : head + max(0, pos_hi / kTileKeys - main0 + 1);
@@ -401,10 +401,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (lane == 0) mbar_arrive(s_free);
         if (cut) {
           // a row's visible keys as bits: up to its position, and in the window
-          // or among the sinks
+          // or among the sinks. (hi - window may wrap where hi <= 0: nothing is
+          // seen then, whatever lo is.)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int hi = pos[i] - key0 + 1, lo = w.window > 0 ? hi - w.window : 0;
+            const int hi = pos[i] - key0 + 1;
+            const int lo = w.window > 0 ? static_cast<int>(static_cast<uint32_t>(hi) - w.window) : 0;
             const int si = w.sinks - key0;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {

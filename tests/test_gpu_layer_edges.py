@@ -91,3 +91,17 @@ def test_row_starts_that_do_not_ascend_stay_inside_the_cache(cuda_device):
         for b, n in enumerate(lens.tolist()):  # nor past a length inside the table
             flat = kc[2 * b:2 * b + 2].transpose(1, 2).reshape(2 * page, -1)
             assert not flat[n:].any()
+
+
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 0), (2 ** 31 - 1, 4), (2 ** 40, 2 ** 40),
+                                          (2 ** 31 - 8, 2 ** 31 - 1)])
+@pytest.mark.parametrize("seqs", [[(10, 4), (300, 100), (5, 5)], [(40, 4), (1, 4000), (6, 1000)]])
+def test_windows_as_wide_as_can_be(cuda_device, window, sinks, seqs):
+    # as good as none, also for new tokens whose positions lie below zero
+    c = Cache(seqs, 2, 128, 16, F16, cuda_device)
+    q = _randn((c.starts[-1], 4, 128), F16, cuda_device, 3)
+    out = cawq.attention_prefill(q, c.k, c.v, c.table, c.lens, c.q_start, window=window, sinks=sinks)
+    ref, tol = attention_ref(q, c)
+    assert_within(out, ref, tol)
+    one = cawq.attention_decode(q[:len(seqs)], c.k, c.v, c.table, c.lens, window=window, sinks=sinks)
+    assert torch.equal(one, cawq.attention_decode(q[:len(seqs)], c.k, c.v, c.table, c.lens))
