@@ -521,7 +521,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int d = 1; d < 4; d <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
-          inv[i] = m[i] != -INFINITY ? 1.f / l[i] : 0.f;  // no key seen: zeros
+          // without a maximum the sum is 0, no key seen, or NaN, a query that is
+          // not finite: the row's output too
+          inv[i] = m[i] != -INFINITY ? 1.f / l[i] : l[i];
           const uint32_t p = p0 + 128 * half + r0 + 8 * i, tok = w.by_group.div(have[i] ? p : 0u);
           dst[i] = a.out + (first + tok) * a.ld_o +
                    static_cast<int64_t>(hk * w.group + p - tok * w.group) * (2 * D);
@@ -543,7 +545,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const float* e = o + 4 * (4 * q + k) + 2 * i;
-                v[k] = m[i] != -INFINITY ? pack2<DT>(e[0] * inv[i], e[1] * inv[i]) : 0u;
+                v[k] = inv[i] != 0.f ? pack2<DT>(e[0] * inv[i], e[1] * inv[i]) : 0u;
               }
               quad_transpose(v, t4);
               if (have[i])

@@ -414,7 +414,8 @@ cawq_status cawq_rope_append(const void* q, const void* k, const void* v, const 
  * over the visible positions j of the token's sequence: j <= pos, and with
  * window > 0 also j > pos - window or j < sinks (the first `sinks` tokens
  * stay visible). Query head h reads kv head h / (n_q / n_kv). A token that
- * sees nothing gets zeros. Scores, the running maximum and sum and the output
+ * sees nothing gets zeros; a query row that is not finite gives NaN in its own
+ * row of out. Scores, the running maximum and sum and the output
  * sums are fp32; the weights of the second product are rounded to `dtype`.
  * q and out: [tokens, n_q, head_dim], token strides in elements (0 = dense),
  * CAWQ_F16 or CAWQ_BF16. workspace: cawq_attention_workspace() bytes of device

@@ -105,3 +105,31 @@ def test_windows_as_wide_as_can_be(cuda_device, window, sinks, seqs):
     assert_within(out, ref, tol)
     one = cawq.attention_decode(q[:len(seqs)], c.k, c.v, c.table, c.lens, window=window, sinks=sinks)
     assert torch.equal(one, cawq.attention_decode(q[:len(seqs)], c.k, c.v, c.table, c.lens))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("seqs", [[(300, 300), (70, 500)], [(2, 3000)], [(1, 5000), (300, 310), (0, 4)],
+                                  [(1, 700), (1, 60), (1, 3000)]])
+def test_queries_that_are_not_finite_give_nan(cuda_device, dtype, d, seqs):
+    # whichever kernel takes the row, and no other row
+    c = Cache(seqs, 2, d, 16, dtype, cuda_device, seed=d)
+    q = _randn((c.starts[-1], 8, d), dtype, cuda_device, 1)
+    calls = [lambda x: cawq.attention_prefill(x, c.k, c.v, c.table, c.lens, c.q_start)]
+    if all(n == 1 for n, _ in seqs):
+        calls.append(lambda x: cawq.attention_decode(x, c.k, c.v, c.table, c.lens))
+    nan, inf = float("nan"), float("inf")
+    tokens = c.starts[-1]
+    hit = torch.zeros((tokens, 8), dtype=torch.bool, device=cuda_device)
+    bad = q.clone()
+    # (token, head, value): past the first tokens, so that the infinite scores
+    # of a row have both signs
+    for t, h, x in ((tokens - 1, 0, nan), (tokens - 1, 7, inf), (0 if seqs[0][1] > 600 else 90, 3, -inf),
+                    (tokens // 2, 5, nan)):
+        t = min(t, tokens - 1)
+        bad[t, h, (7 * h + 5) % d] = x
+        hit[t, h] = True
+    for call in calls:
+        want, got = call(q), call(bad)
+        assert got[hit].isnan().all()
+        assert torch.equal(got[~hit], want[~hit])
