@@ -135,8 +135,9 @@ struct AttWork {
     s.len = kv.len(b);
     const int pos = s.len - s.count;  // of the first new token
     s.start = window_start(pos);
-    s.head = min(sinks, s.start);
-    s.keys = s.len - s.start + s.head;
+    const int end = min(s.len, kv.cap());
+    s.head = min(min(sinks, s.start), end);
+    s.keys = max(0, end - s.start) + s.head;
     s.row_tiles = (static_cast<uint32_t>(s.count) * group + row_tile - 1) / row_tile;
     s.tiles = s.count > 0 && (!shared || s.count * group <= kAttFewRows)
                   ? max(1, (s.keys + kAttKeys - 1) / kAttKeys)
@@ -170,7 +171,7 @@ struct AttLoad {
     AttLoad a = {0, 0};
     if (count <= 0 || len <= 0) return a;
     const int64_t rows = static_cast<int64_t>(count) * w.group;
-    int64_t n = len;
+    int64_t n = min(len, w.kv.cap());
     if (w.window > 0) n = min(n, static_cast<int64_t>(w.window) + w.sinks + count);
     const bool few = rows <= kAttFewRows;
     if (few) a.longest = static_cast<uint32_t>(n);

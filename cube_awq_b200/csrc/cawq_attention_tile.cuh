@@ -328,9 +328,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int pos_lo = shift + static_cast<int>(w.by_group.div(p0));
   const int pos_hi = shift + static_cast<int>(w.by_group.div(p1 - 1));
   const int start = w.window_start(pos_lo);
-  const int head = (min(w.sinks, start) + kTileKeys - 1) / kTileKeys;  // blocks that hold sinks
+  // past the table's end there is nothing: no blocks, and keys of the last one
+  // that lie there count as a page that is missing
+  const int last = min(pos_hi, w.kv.cap() - 1);
+  const int head = (min(min(w.sinks, start), last + 1) + kTileKeys - 1) / kTileKeys;  // blocks that hold sinks
   const int main0 = max(start / kTileKeys, head);
-  const int nb = pos_hi < 0 ? 0 : head + max(0, pos_hi / kTileKeys - main0 + 1);
+  const int nb = last < 0 ? 0 : head + max(0, last / kTileKeys - main0 + 1);
   auto block_key = [&](int j) { return (j < head ? j : main0 + j - head) * kTileKeys; };
 
   const uint32_t tmem = *tmem_slot;
@@ -655,7 +658,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                (x.key + static_cast<int>(box_keys) > start || x.key < sinks);
       const uint32_t pg = x.need ? w.kv.page.div(x.key) : 0u;
       x.in_page = x.need ? x.key - static_cast<int>(pg * w.kv.page.d) : 0;
-      x.page = x.need ? table[pg] : -1;
+      x.page = x.need && pg < w.kv.width ? table[pg] : -1;
       return x;
     };
     auto find = [&](Box& x) {

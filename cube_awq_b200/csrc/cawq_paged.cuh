@@ -37,11 +37,14 @@ struct PagedView {
   uint32_t pages, width, batch, n_kv;
   FastDiv page;
 
-  // tokens of sequence b, bounded by what its table row can hold
+  // positions that a table row can hold
+  __device__ __forceinline__ int cap() const { return static_cast<int>(width * page.d); }
+  // tokens of sequence b. More than cap() of them set the error bit: the new
+  // tokens' positions follow from the length as it is, keys end at cap().
   __device__ __forceinline__ int len(uint32_t b) const {
-    const int n = lens[b], most = static_cast<int>(width * page.d);
-    if (n > most) atomicOr(&g_cawq_device_error, kErrCache);
-    return max(0, min(n, most));
+    const int n = lens[b];
+    if (n > cap()) atomicOr(&g_cawq_device_error, kErrCache);
+    return max(0, n);
   }
   // rows [first, first + count) of the call's tensors are sequence b's
   __device__ __forceinline__ void rows(uint32_t b, uint32_t tokens, int* first, int* count) const {
@@ -72,10 +75,10 @@ struct PagedView {
     }
   }
   // byte offset of position j of sequence b, head h (the same in k and v);
-  // -1 (and the error bit) if its page is none of the cache's. j < len(b).
+  // -1 (and the error bit) if its page is past the table or none of the cache's.
   __device__ __forceinline__ int64_t offset(uint32_t b, uint32_t h, uint32_t j) const {
     const uint32_t p = page.div(j);
-    const int32_t pg = table[b * ld_table + p];
+    const int32_t pg = p < width ? table[b * ld_table + p] : -1;
     if (static_cast<uint32_t>(pg) >= pages) {
       atomicOr(&g_cawq_device_error, kErrCache);
       return -1;

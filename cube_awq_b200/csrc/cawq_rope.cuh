@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(kRopeThreads)
     int first, count;
     kv.rows(b, tokens, &first, &count);
     // a row before q_start[0], or one that starts out of order left outside its
-    // sequence, has no place: with it pos < len(b), which offset() relies on
+    // sequence, has no place
     if (static_cast<int>(t) >= first && static_cast<int>(t) < first + count)
       pos = kv.len(b) - count + static_cast<int>(t) - first;
   }

@@ -377,8 +377,8 @@ cawq_status cawq_rms_norm_fp8(const void* x, const void* weight, const void* res
  * seq_lens, q_start and block_table are device memory, so their values are
  * checked by the kernels: a page outside [0, pages) or a position past the
  * table is skipped (no read, no write) and sets bit 2 of the device error
- * word; a new token whose position is negative (an empty slot of a batch)
- * sees no key.
+ * word (new tokens keep the positions that seq_lens gives them); a new token
+ * whose position is negative (an empty slot of a batch) sees no key.
  */
 typedef struct cawq_paged_kv {
   void* k;

@@ -133,3 +133,97 @@ def test_queries_that_are_not_finite_give_nan(cuda_device, dtype, d, seqs):
         want, got = call(q), call(bad)
         assert got[hit].isnan().all()
         assert torch.equal(got[~hit], want[~hit])
+
+
+def test_rope_past_the_table_is_skipped(cuda_device):
+    # a table of 4 pages of 16: position 64 and later have no slot
+    q, k, v, rope = _rope_args(cuda_device, 3)
+    kc = _randn((13, 2, 16, 64), F16, cuda_device, 7)
+    vc = _randn((13, 2, 16, 64), F16, cuda_device, 8)
+    table = torch.arange(12, dtype=torch.int32, device=cuda_device).view(3, 4)
+    kk, vv = kc.clone(), vc.clone()
+    out = cawq.rope_append(q, k, v, rope, kc, vc, table, _i32([65, 64, 100], cuda_device))
+    assert cawq.device_error() == 4
+    for a, b in ((kc, kk), (vc, vv)):  # the second one's slot alone is written
+        b[7, :, 15] = a[7, :, 15]
+        assert torch.equal(a, b)
+    assert torch.equal(vc[7, :, 15], v[1])
+    # q turns by its true position
+    far = torch.zeros((3, 13), dtype=torch.int32, device=cuda_device)
+    far[:, :4] = 12
+    want = cawq.rope_append(q, k, v, rope, kk, vv, far, _i32([65, 64, 100], cuda_device))
+    assert torch.equal(out, want)
+    # of a run of new tokens those that have a slot are stored in it
+    kc2, vc2 = kk.clone(), vv.clone()
+    cawq.rope_append(q, k, v, rope, kc2, vc2, table[:1], _i32([66], cuda_device), q_start=_i32([0, 3], cuda_device))
+    assert cawq.device_error() == 4
+    assert torch.equal(vc2[3, :, 15], v[0])
+    kc2[3, :, 15], vc2[3, :, 15] = kk[3, :, 15], vv[3, :, 15]
+    assert torch.equal(kc2, kk) and torch.equal(vc2, vv)
+
+
+class _Cut(Cache):
+    """A cache whose tables hold `slots` positions, given to calls whose
+    sequences are longer: their other keys and values do not exist."""
+
+    def __init__(self, seqs, slots, hkv, d, page, dtype, device, seed=0):
+        super().__init__([(n, min(t, slots)) for n, t in seqs], hkv, d, page, dtype, device, seed=seed,
+                         table_extra=0)
+        assert self.table.shape[1] * page == slots
+        self.true = [t for _, t in seqs]
+        self.lens = _i32(self.true, device)
+
+
+def _cut_ref(q, c, window, sinks):
+    """attention_ref with the queries at their true positions, keys up to the table's end."""
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    for i, ((n, have), true) in enumerate(zip(c.seqs, c.true)):
+        rows = slice(c.starts[i], c.starts[i] + n)
+        for t in range(n):
+            pos = true - n + t
+            seen = [j for j in range(min(pos + 1, have)) if not window or j > pos - window or j < sinks]
+            one = Cache.__new__(Cache)
+            one.seqs, one.starts, one.k = [(1, len(seen))], [0, 1], c.k
+            one.kd, one.vd = [c.kd[i][seen]], [c.vd[i][seen]]
+            r = rows.start + t
+            out[r:r + 1], tol[r:r + 1] = attention_ref(q[r:r + 1], one)
+    return out, tol
+
+
+@pytest.mark.parametrize("page,slots", [(16, 336), (8, 72), (64, 640)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 0), (40, 7), (700, 100)])
+def test_attention_past_the_table(cuda_device, page, slots, d, window, sinks):
+    # positions are the true ones, keys end with the table
+    seqs = [(3, slots + 1), (20, slots + 6), (40, slots + 40), (2, slots + 1000), (70, slots), (5, 9),
+            (1, 2 ** 31 - 1), (33, 2 ** 30)]
+    c = _Cut(seqs, slots, 2, d, page, BF16, cuda_device, seed=slots)
+    q = _randn((c.starts[-1], 8, d), BF16, cuda_device, 1)
+    out = cawq.attention_prefill(q, c.k, c.v, c.table, c.lens, c.q_start, window=window, sinks=sinks)
+    assert cawq.device_error() == 4
+    ref, tol = _cut_ref(q, c, window, sinks)
+    assert_within(out, ref, tol)
+    for part in ([1], [2], [3], [7]):  # alone, so that either kernel takes them
+        i = part[0]
+        rows = slice(c.starts[i], c.starts[i + 1])
+        out = cawq.attention_prefill(q[rows], c.k, c.v, c.table[i:i + 1], c.lens[i:i + 1],
+                                     _i32([0, seqs[i][0]], cuda_device), window=window, sinks=sinks)
+        assert_within(out, ref[rows], tol[rows])
+    assert cawq.device_error() == 4
+    one = _Cut([(1, t) for _, t in seqs], slots, 2, d, page, BF16, cuda_device, seed=slots + 1)
+    out = cawq.attention_decode(q[:len(seqs)], one.k, one.v, one.table, one.lens, window=window, sinks=sinks)
+    assert cawq.device_error() == 4
+    ref, tol = _cut_ref(q[:len(seqs)], one, window, sinks)
+    assert_within(out, ref, tol)
+
+
+def test_many_rows_past_the_table(cuda_device):
+    # a long run whose first tokens have slots and whose last ones have none
+    c = _Cut([(500, 800), (300, 700)], 640, 1, 128, 16, F16, cuda_device)
+    q = _randn((c.starts[-1], 4, 128), F16, cuda_device, 1)
+    for window, sinks in ((0, 0), (100, 5)):
+        out = cawq.attention_prefill(q, c.k, c.v, c.table, c.lens, c.q_start, window=window, sinks=sinks)
+        assert cawq.device_error() == 4
+        ref, tol = _cut_ref(q, c, window, sinks)
+        assert_within(out, ref, tol)
