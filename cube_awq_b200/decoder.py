@@ -70,16 +70,18 @@ class AWQDecoderLayer:
         if stream is None:
             stream = x
         q, k, v = self.qkv(h)
-        heads = (tokens, -1, self.head_dim)
-        q = rope_append(q.view(heads), k.view(heads), v.view(heads), rope, k_cache, v_cache,
-                        block_table, seq_lens, q_start=q_start, out=q.view(heads))
+        q = q.view(tokens, self.n_q, self.head_dim)
+        heads = (tokens, self.n_kv, self.head_dim)
+        q = rope_append(q, k.view(heads), v.view(heads), rope, k_cache, v_cache, block_table,
+                        seq_lens, q_start=q_start, out=q)
         if q_start is None:
             a = attention_decode(q, k_cache, v_cache, block_table, seq_lens, window=self.window,
                                  sinks=self.sinks)
         else:
             a = attention_prefill(q, k_cache, v_cache, block_table, seq_lens, q_start,
                                   window=self.window, sinks=self.sinks)
-        h, stream = rms_norm(self.o(a.view(tokens, -1)), self.post_norm, self.eps, residual=stream)
+        a = self.o(a.view(tokens, self.n_q * self.head_dim))
+        h, stream = rms_norm(a, self.post_norm, self.eps, residual=stream)
         return self.down(self.gate_up(h)), stream
 
     __call__ = forward

@@ -124,3 +124,19 @@ def test_sizes_that_do_not_fit_are_refused(cuda_device):
             cawq.AWQDecoderLayer(*args, *heads)
     with pytest.raises(ShapeError):
         cawq.AWQDecoderLayer(layer.input_norm[:256], *args[1:], NQ, NKV, D)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_no_tokens(cuda_device, dtype):
+    # an empty batch, and a batch whose sequences have no new tokens
+    layer, *_ = _layer(dtype, cuda_device, None, 0)
+    x = torch.empty((0, HIDDEN), dtype=dtype, device=cuda_device)
+    kc = torch.ones((4, NKV, 16, D), dtype=dtype, device=cuda_device)
+    vc, rope = kc.clone(), cawq.rope_table(32, D, device=cuda_device)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=cuda_device)  # noqa: E731
+    for r in (x, None):
+        for table, lens, starts in ((i32(0, 2), i32(0), None), (i32(0, 2), i32(0), i32(1)),
+                                    (i32(2, 2), i32(2) + 3, i32(3))):
+            y, h = layer(x, r, rope, kc, vc, table, lens, q_start=starts)
+            assert y.shape == h.shape == (0, HIDDEN) and y.dtype == h.dtype == dtype
+    assert (kc == 1).all() and (vc == 1).all() and cawq.device_error() == 0
