@@ -25,6 +25,9 @@ namespace cawq {
 
 constexpr int kNormThreads = 256;  // of CTAs with a row a warp, and for the longest rows
 constexpr float kE4m3Max = 448.f;
+// Below this largest |y| of a row (448 / FLT_MAX is 1.3e-36) 448 / max |y| may
+// pass fp32's range: y and the maximum are multiplied by 2^64 first, exactly.
+constexpr float kTinyTop = 0x1p-118f, kTinyUp = 0x1p64f;
 
 // Sum (or maximum) of one value per thread over the block; every thread gets it.
 template <bool MAX>
@@ -97,19 +100,20 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormArgs<DT> a) {
   each([&](uint32_t, float v) { sum += v * v; });
   sum = block_reduce<false>(sum, scratch);
   const float rs = 1.f / sqrtf(sum / static_cast<float>(a.d) + a.eps);
-  float inv = 0.f;
+  float inv = 0.f, up = 1.f;
   if constexpr (FP8) {
     float top = 0.f;
     each([&](uint32_t i, float v) { top = fmaxf(top, fabsf(v * rs * D::to_f32(a.w[i]))); });
     top = block_reduce<true>(top, scratch);
-    inv = top > 0.f ? kE4m3Max / top : 0.f;
     if (threadIdx.x == 0) a.scales[row] = top / kE4m3Max;
+    if (top < kTinyTop) up = kTinyUp;
+    inv = top > 0.f ? kE4m3Max / (top * up) : 0.f;
   }
   each([&](uint32_t i, float u) {
     const float v = u * rs * D::to_f32(a.w[i]);
     if (a.res_out) a.res_out[row * a.ld_ro + i] = D::from_f32(u);
     if constexpr (FP8)
-      static_cast<__nv_fp8_e4m3*>(a.y)[row * a.ld_y + i] = __nv_fp8_e4m3(v * inv);
+      static_cast<__nv_fp8_e4m3*>(a.y)[row * a.ld_y + i] = __nv_fp8_e4m3(v * up * inv);
     else
       static_cast<T*>(a.y)[row * a.ld_y + i] = D::from_f32(v);
   });
@@ -207,8 +211,15 @@ __global__ void __launch_bounds__(WARP || VPT == 4 ? kNormThreads : VPT == 1 ? 1
   }
   if constexpr (FP8) {
     top = reduce(top, std::true_type{});
-    const float inv = top > 0.f ? kE4m3Max / top : 0.f;
     if (lane == 0) a.scales[row] = top / kE4m3Max;
+    if (top < kTinyTop) {
+      top *= kTinyUp;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int k = 0; k < N; ++k) h[i][k] *= kTinyUp;
+    }
+    const float inv = top > 0.f ? kE4m3Max / top : 0.f;
     uint8_t* o = static_cast<uint8_t*>(a.y) + row * a.ld_y;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {

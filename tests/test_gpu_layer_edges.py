@@ -227,3 +227,30 @@ def test_many_rows_past_the_table(cuda_device):
         assert cawq.device_error() == 4
         ref, tol = _cut_ref(q, c, window, sinks)
         assert_within(out, ref, tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [64, 520, 1001, 8192, 17001])
+@pytest.mark.parametrize("size", [1e-40, 1e-38, 1e-36, 1.3e-36, 1.4e-36])
+def test_rms_norm_fp8_of_rows_that_are_hardly_there(cuda_device, dtype, d, size):
+    # 448 / max |y| passes the largest fp32 below 1.3e-36. eps is large, so that
+    # y = x * weight to fp32's precision, and the weights put |y| near `size`.
+    x = _randn((5, d), dtype, cuda_device, 1)
+    x[:, ::7] = 0
+    x[4] = 0
+    w = (torch.rand(d, generator=torch.Generator(device=cuda_device).manual_seed(2),
+                    device=cuda_device) + 0.5).mul_(size).to(dtype)
+    y8, s, _ = cawq.rms_norm_fp8(x, w, 1.0)
+    h = x.double()
+    y = h / (h.square().mean(dim=1, keepdim=True) + 1.0).sqrt() * w.double()
+    scale = y.abs().amax(dim=1) / 448
+    tiny = 2.0 ** -149  # the grid of fp32 values this small: y, the largest, the scale
+    assert_within(s, scale, scale * 1e-4 + 1.1 * tiny, "scale")
+    assert not s[4].any() and not y8[4].float().any()
+    ratio = torch.where(scale[:, None] > 0, y / scale[:, None], 0.0)
+    # e4m3: half a step is 2^-4 of the value, 2^-10 below the normal range; y and
+    # the maximum are off by up to a step of their grid each, which the ratio scales
+    grid = torch.where(scale > 0, 1.1 * tiny / scale, 0.0)[:, None]
+    tol = torch.maximum(ratio.abs() * 2.0 ** -4, torch.tensor(2.0 ** -10, dtype=torch.float64)) * 1.01 \
+        + ratio.abs() * (1e-4 + grid / 448) + grid
+    assert_within(y8.double(), ratio, tol, "y8")
