@@ -29,13 +29,20 @@ constexpr float kE4m3Max = 448.f;
 // pass fp32's range: y and the maximum are multiplied by 2^64 first, exactly.
 constexpr float kTinyTop = 0x1p-118f, kTinyUp = 0x1p64f;
 
+// The larger one, NaN where either is (fmaxf would pass it by).
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Sum (or maximum) of one value per thread over the block; every thread gets it.
 template <bool MAX>
 __device__ __forceinline__ float warp_reduce(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = MAX ? fmaxf(v, u) : v + u;
+    v = MAX ? max_or_nan(v, u) : v + u;
   }
   return v;
 }
@@ -47,7 +54,7 @@ __device__ __forceinline__ float block_reduce(float v, float* scratch) {
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
   __syncthreads();
   v = scratch[0];
-  for (int i = 1; i < warps; ++i) v = MAX ? fmaxf(v, scratch[i]) : v + scratch[i];
+  for (int i = 1; i < warps; ++i) v = MAX ? max_or_nan(v, scratch[i]) : v + scratch[i];
   return v;
 }
 
@@ -103,7 +110,7 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormArgs<DT> a) {
   float inv = 0.f, up = 1.f;
   if constexpr (FP8) {
     float top = 0.f;
-    each([&](uint32_t i, float v) { top = fmaxf(top, fabsf(v * rs * D::to_f32(a.w[i]))); });
+    each([&](uint32_t i, float v) { top = max_or_nan(top, fabsf(v * rs * D::to_f32(a.w[i]))); });
     top = block_reduce<true>(top, scratch);
     if (threadIdx.x == 0) a.scales[row] = top / kE4m3Max;
     if (top < kTinyTop) up = kTinyUp;
@@ -205,7 +212,7 @@ __global__ void __launch_bounds__(WARP || VPT == 4 ? kNormThreads : VPT == 1 ? 1
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         h[i][k] = h[i][k] * rs * w[k];
-        if constexpr (FP8) top = fmaxf(top, fabsf(h[i][k]));
+        if constexpr (FP8) top = max_or_nan(top, fabsf(h[i][k]));
       }
     }
   }

@@ -357,7 +357,7 @@ cawq_status cawq_rms_norm(const void* x, const void* weight, const void* residua
 /*
  * The same with y in 8 bits: scales[row] = max |y| / 448 (fp32) and
  * y8 = e4m3(y / scales[row]), rounded to nearest even from the fp32 y; a row
- * of zeros has scale 0. y8 must not overlap x.
+ * of zeros has scale 0, one that holds a NaN scale NaN. y8 must not overlap x.
  */
 cawq_status cawq_rms_norm_fp8(const void* x, const void* weight, const void* residual, void* y8,
                               float* scales, void* residual_out, size_t rows, size_t d,

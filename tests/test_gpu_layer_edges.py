@@ -254,3 +254,20 @@ def test_rms_norm_fp8_of_rows_that_are_hardly_there(cuda_device, dtype, d, size)
     tol = torch.maximum(ratio.abs() * 2.0 ** -4, torch.tensor(2.0 ** -10, dtype=torch.float64)) * 1.01 \
         + ratio.abs() * (1e-4 + grid / 448) + grid
     assert_within(y8.double(), ratio, tol, "y8")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,d", [(6, 64), (600, 64), (600, 1000), (6, 4096), (6, 1001), (6, 17001)])
+def test_rms_norm_fp8_of_rows_that_are_not_finite(cuda_device, dtype, rows, d):
+    # the largest |y| of a row that holds a NaN is NaN, and so is its scale
+    x, w = _randn((rows, d), dtype, cuda_device, 1), _randn((d,), dtype, cuda_device, 2)
+    clean = cawq.rms_norm_fp8(x, w)
+    bad = x.clone()
+    bad[1, d - 1], bad[3, d // 2], bad[5, 0] = float("nan"), float("inf"), -float("inf")
+    y8, s, _ = cawq.rms_norm_fp8(bad, w)
+    hit = torch.zeros(rows, dtype=torch.bool, device=cuda_device)
+    hit[[1, 3, 5]] = True
+    assert s[hit].isnan().all() and y8[1].float().isnan().all()
+    assert y8[3, d // 2].float().isnan() and y8[5, 0].float().isnan()
+    assert torch.equal(s[~hit], clean[1][~hit])
+    assert torch.equal(y8[~hit].view(torch.uint8), clean[0][~hit].view(torch.uint8))
