@@ -245,11 +245,14 @@ __device__ __forceinline__ void pick_tile_of_many(const AttWork& w, uint32_t ind
 }
 
 // Pages as heads: how many head strides a page stride is; 0 where the two do
-// not make one dimension (the split kernel then takes the call).
+// not make one dimension, or where a dimension that is walked has a stride of 0
+// (a broadcast view; a tensor map is not made of one). The split kernel then
+// takes the call.
 inline uint64_t tile_heads_per_page(const PagedView& kv) {
-  if (kv.pages == 0) return 0;
+  if (kv.pages == 0 || kv.st <= 0 || (kv.n_kv > 1 && kv.sh <= 0) || (kv.pages > 1 && kv.sp <= 0))
+    return 0;
   if (kv.n_kv == 1 || kv.pages == 1) return kv.n_kv;
-  if (kv.sh <= 0 || kv.sp % kv.sh != 0 || kv.sp / kv.sh < static_cast<int64_t>(kv.n_kv)) return 0;
+  if (kv.sp % kv.sh != 0 || kv.sp / kv.sh < static_cast<int64_t>(kv.n_kv)) return 0;
   const uint64_t per = static_cast<uint64_t>(kv.sp / kv.sh);
   return per * (kv.pages + 1) < (1ull << 31) ? per : 0;
 }

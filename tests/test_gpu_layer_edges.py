@@ -271,3 +271,24 @@ def test_rms_norm_fp8_of_rows_that_are_not_finite(cuda_device, dtype, rows, d):
     assert y8[3, d // 2].float().isnan() and y8[5, 0].float().isnan()
     assert torch.equal(s[~hit], clean[1][~hit])
     assert torch.equal(y8[~hit].view(torch.uint8), clean[0][~hit].view(torch.uint8))
+
+
+@pytest.mark.parametrize("pages,hkv", [(1, 2), (1, 1), (5, 1), (5, 2)])
+@pytest.mark.parametrize("what", ["heads", "pages", "slots"])
+def test_broadcast_caches(cuda_device, pages, hkv, what):
+    # views with a stride of 0: they may be read, whichever kernel takes the call
+    page, d = 64, 128
+    shape = dict(heads=(pages, 1, page, d), pages=(1, hkv, page, d), slots=(pages, hkv, 1, d))[what]
+    k, v = (_randn(shape, F16, cuda_device, s).expand(pages, hkv, page, d) for s in (1, 2))
+    total = pages * page - 3
+    q = _randn((min(total, 200), 4 * hkv, d), F16, cuda_device, 3)
+    n = q.shape[0]
+    table = torch.arange(pages, dtype=torch.int32, device=cuda_device)[None]
+    lens, q_start = _i32([total], cuda_device), _i32([0, n], cuda_device)
+    c = Cache.__new__(Cache)
+    c.seqs, c.starts, c.k = [(n, total)], [0, n], k
+    c.kd, c.vd = ([x.transpose(1, 2).reshape(pages * page, hkv, d)[:total]] for x in (k, v))
+    ref, tol = attention_ref(q, c)
+    assert_within(cawq.attention_prefill(q, k, v, table, lens, q_start), ref, tol)
+    out = cawq.attention_decode(q[-1:], k, v, table, lens)
+    assert_within(out, ref[-1:], tol[-1:])
