@@ -203,7 +203,10 @@ static cawq_status attention(const void* q, void* out, const cawq_paged_kv* kv, 
                               static_cast<int>(std::min(window, kMaxInt)),
                               static_cast<int>(std::min(sinks, kMaxInt)), dtype, workspace,
                               dev.sm_count, dev.device, static_cast<cudaStream_t>(stream)};
-  const PagedView view = paged_view(*kv, 2, decode);
+  PagedView view = paged_view(*kv, 2, decode);
+  // copies of no bytes, of keys that are masked, name the cache's first address:
+  // of a cache without pages, which may have none, another valid one
+  if (kv->pages == 0) view.k = view.v = static_cast<char*>(const_cast<void*>(q));
   // Sequences of few query rows go to the split kernel where splitting their
   // keys pays, the others to the tile kernel (AttLoad). The lengths are the
   // device's; the host goes by what it knows, the rows in all and the most keys

@@ -292,3 +292,22 @@ def test_broadcast_caches(cuda_device, pages, hkv, what):
     assert_within(cawq.attention_prefill(q, k, v, table, lens, q_start), ref, tol)
     out = cawq.attention_decode(q[-1:], k, v, table, lens)
     assert_within(out, ref[-1:], tol[-1:])
+
+
+@pytest.mark.parametrize("pages,width", [(0, 0), (0, 3), (4, 0)])
+def test_caches_and_tables_that_hold_nothing(cuda_device, pages, width):
+    kc = torch.ones((pages, 2, 16, 64), dtype=F16, device=cuda_device)
+    vc = kc.clone()
+    table = torch.zeros((3, width), dtype=torch.int32, device=cuda_device)
+    q, k, v, rope = _rope_args(cuda_device, 3)
+    for lens, error in (([0, 0, 0], 0), ([0, 20, 1], 4)):
+        lens = _i32(lens, cuda_device)
+        assert not cawq.attention_decode(q, kc, vc, table, lens).any()
+        assert cawq.device_error() == error
+        for starts in ([0, 1, 2, 3], [0, 0, 3, 3]):
+            assert not cawq.attention_prefill(q, kc, vc, table, lens, _i32(starts, cuda_device)).any()
+            assert cawq.device_error() == error
+        out = cawq.rope_append(q, k, v, rope, kc, vc, table, lens)
+        assert cawq.device_error() == error
+        assert out[1].any() == bool(error) and not out[0].any()
+        assert (kc == 1).all() and (vc == 1).all()
