@@ -9,7 +9,7 @@
 // 2^(m2 - M) sum2, the same for the outputs.
 //
 // Bound by the cache's bytes (one sequence of 131072 tokens, 64 / 8 heads, bf16:
-// 537 MB in 89 us, 6.0 TB/s) and, below some 100 MB, by what a launch costs at
+// 537 MB in 88-91 us, 5.9-6.1 TB/s) and, below some 100 MB, by what a launch costs at
 // its ends, 8 us with the join (64 sequences of 1 to 8000 tokens, 28 / 4 heads:
 // 133 MB in 33 us): every visible key and value is read once per tile of query
 // rows that shares its kv head. A row tile is NR = 8 or 16 rows
@@ -30,8 +30,11 @@
 // so that ldmatrix reads without bank conflicts; a masked row is filled with
 // zeros and never read). The stream runs on across row tiles. With mma.sync
 // m16n8k16 the keys are the MMA's rows: S^T = K Q^T needs only N = 8 columns
-// for 8 query rows; the weights, rounded to the operand type, turn in
-// registers (movmatrix) into the B operand of O^T += V^T P^T.
+// for 8 query rows; the weights, rounded to the operand type, which is what the
+// instruction takes, turn in registers (movmatrix) into the B operand of O^T +=
+// V^T P^T. The sums take them unrounded. Against 64 bits the output's error is
+// 2.0e-3 in bf16, 2.2e-4 in f16, where weights of 32 bits leave 1.6e-3 and 2.1e-4
+// (relative, 131072 and 1000 tokens).
 #pragma once
 
 #include "cawq_norm.cuh"
@@ -154,11 +157,16 @@ struct AttWork {
 // ns, kPole in that time; the split kernel reads a sequence's keys once per row
 // tile of 16, but no CTA waits for the longest. So it gains where the longest
 // sequence of few rows, less what its two launches cost, has more keys than all
-// row tiles together have per kPole. us split / tiles (bf16, D = 128, 8 kv heads,
-// all of 1000 / 4000 / 16000 tokens): 1 sequence of 16 rows 15 / 17 / 27 against
-// 15 / 43 / 150, of 128 rows 20 / 35 / 93 against 16 / 44 / 152; 8 of 16 rows
-// 20 / 39 / 99 against 16 / 46 / 155, of 64 rows 44 / 108 / 351 against
-// 17 / 46 / 156; 32 of 16 rows and 1 to 8000 tokens 33 against 81.
+// row tiles together have per kPole. us split against tiles (bf16, 8 kv heads,
+// all of 1000 / 4000 / 16000 tokens), D = 128: 1 sequence of 16 rows 14 / 17 / 27
+// against 15 / 42 / 149, of 128 rows 20 / 35 / 93 against 16 / 44 / 151; 8 of 16
+// rows 21 / 39 / 100 against 22 / 52 / 160, of 64 rows 48 / 110 / 356 against
+// 23 / 52 / 160; 32 of 16 rows and 1 to 8000 tokens 50 against 86. D = 64, whose
+// blocks of keys take a tile as long and the split kernel not much less: 13 / 15 /
+// 21 against 14 / 42 / 150, 17 / 30 / 77 against 15 / 43 / 152; 17 / 32 / 81
+// against 20 / 50 / 160, 40 / 90 / 290 against 21 / 51 / 160; 41 against 85. The
+// rule picks the faster of the two in all of them but 8 of 16 rows and 1000
+// tokens, where it costs 3 us (D = 64) or nothing.
 struct AttLoad {
   static constexpr uint32_t kPole = 111, kLaunch = 850;
   uint64_t keys;     // of the row tiles, or tiles, of all sequences

@@ -5,9 +5,11 @@
 // token's position: (a, b) -> (a c - b s, b c + a s), in fp32 with one
 // rounding.
 //
-// Bound by bytes for prompts (3083 tokens, 28 / 4 heads, bf16: 58 MB in 14.7 us,
-// 4.0 TB/s, with 2-3 us of launch and look-ups in it) and by latency for single
-// tokens (64 tokens, 32 / 32 heads, f16: 2.7 us). One CTA per token, a thread
+// Prompts (3083 tokens, 28 / 4 heads, bf16: 58 MB in 14.8 us, 3.9 TB/s) wait for
+// the chain that each token's CTA goes through, sequence, length and row starts,
+// page, angles, each load's address from the one before (5.3 cycles of long
+// scoreboard stall an issue), beside 2-3 us of launch; single tokens are latency
+// altogether (64 tokens, 32 / 32 heads, f16: 2.7 us). One CTA per token, a thread
 // per 8 elements of the lower half of a head and the 8 that turn with them, so
 // every access is 16 bytes; its loads go out before the token's sequence,
 // position and page are looked up. (Two heads a thread, and CTAs of 128 or 256,

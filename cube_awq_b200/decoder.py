@@ -12,8 +12,9 @@ rotary decoders that AutoAWQ checkpoints hold:
     h, r  = rms_norm(o(a) + r)
     x     = down(silu(gate(h)) * up(h))
 
-Eight launches a layer for prompts and for single tokens alike (nine where the
-attention of long caches joins its parts in a second one).
+Eight to ten launches a layer: the attention is one of them, two where it splits
+long caches and joins the parts, three where a batch of prompts and short runs
+behind long caches takes both of its forms.
 """
 
 from __future__ import annotations

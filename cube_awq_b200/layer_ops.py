@@ -17,14 +17,17 @@ made whole by
 The cache is a pair of tensors ``k_cache``, ``v_cache`` [pages, n_kv,
 page_size, head_dim] (any strides that are multiples of 8 elements with a unit
 innermost one, the same for both, so one may be a view into a larger pool or
-hold its tokens outermost in a page), with ``block_table`` int32 [batch,
+hold its tokens outermost in a page; but prompts are attended at full speed
+only where the page stride is a multiple of the head stride: heads outermost,
+or pages padded by part of a head, take 4 to 20 times as long), with ``block_table`` int32 [batch,
 table_width] (token j of sequence b is slot j % page_size of page
 ``block_table[b, j // page_size]``) and ``seq_lens`` int32 [batch], the tokens
 of each sequence with the call's own. Several new tokens per sequence come
 with ``q_start`` int32 [batch + 1]: rows ``q_start[b]:q_start[b + 1]`` are the
 last tokens of sequence b. These three live on the GPU and are not read by the
 host: pages and positions outside the cache are skipped by the kernels and
-reported by :func:`device_error` (bit 2).
+reported by :func:`device_error` (bit 2). The [tokens, heads, head_dim] operands
+start on 16 bytes and have token strides that are multiples of 8 elements.
 """
 
 from __future__ import annotations
@@ -148,8 +151,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
                  ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """:func:`rms_norm` with y in 8 bits (cawq_rms_norm_fp8) -> (y8, scales, h):
     scales[...] = max |y| / 448 of a row (fp32), y8 = float8_e4m3fn(y / scale),
-    the operands of an 8-bit product with row scales (a module that AutoAWQ
-    left unquantised, such as lm_head)."""
+    the operands of an 8-bit product with row scales (of a module that AutoAWQ
+    left unquantised, such as lm_head; this package has no such product)."""
     ext = _torch_ext()
     if ext is not None:
         r = ext.rms_norm_fp8(x, weight, eps, residual, out, scales, residual_out)
