@@ -152,3 +152,18 @@ def test_python_layer_refusals(cuda_device):
                         ((z(3, 0), z(0)), {}, ShapeError)]:
         with pytest.raises(kind):
             cawq.rms_norm(*a, **kw)
+
+
+@pytest.mark.parametrize("over,tokens", [(dict(), 3), (dict(batch=1), 1), (dict(q_start=64), 9),
+                                         (dict(table_width=1), 3)])
+def test_short_workspaces_are_refused(over, tokens):
+    kv = _kv(**over)
+    need = _lib.lib().cawq_attention_workspace(ctypes.byref(kv), tokens, 4)
+    assert need > 0
+    for ws, nbytes in ((P, need - 1), (P, 0), (None, need), (ctypes.c_void_p(72), need)):
+        if kv.q_start is None:
+            st = _decode(kv, ws=ws, nbytes=nbytes)
+        else:
+            st = _lib.lib().cawq_attention_prefill(P, P, ctypes.byref(kv), tokens, 4, 0, 0, 1.0, 0, 0,
+                                                   _lib.CAWQ_F16, ws, nbytes, None)
+        assert st == _lib.CAWQ_ERR_INVALID_ARGUMENT and "workspace" in _lib.last_error()
